@@ -102,7 +102,7 @@ def draw(rng):
 def _codes(x):
     """Rows (the last axis) as codes and scales, in the input's precision."""
     top = x.abs().amax(-1)
-    scales = top / 127
+    scales = top * (1 / 127)
     codes = torch.round(x / torch.where(scales > 0, scales, 1).unsqueeze(-1)).clamp(-127, 127)
     return codes, scales
 
