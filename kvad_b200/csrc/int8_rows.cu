@@ -1,0 +1,268 @@
+// Rows held in 8 bits: a row x is codes c (integers of -127 .. 127) and one 32-bit scale s,
+//
+//   s = max_j |x_j| / 127,    c_j = x_j / s rounded to the nearest integer, halves to the even one,    x_j ~ c_j s,
+//
+// so that an entry is at most s / 2 from what it stands for.  (The division by 127 is one 32-bit product with 1/127; the division by s is one.)  A row of zeros (or one so small that s is zero) has the scale 0 and codes 0.
+// A row that holds a number that is not finite has the scale NaN and codes 0: whatever is computed from it is NaN, and says so.
+//
+// kvad_int8_rows: rows as they are, or what an RMS or layer norm makes of them, after a sublayer's result has been added to the stream:
+//
+//   t = x + mult * delta;    y = t / sqrt(mean(t^2) + eps) * w        (layer: t less its mean, + b)
+//
+// One pass: a row's entries stay in the registers of its threads from the sum through both reductions (mean square, maximum) to the
+// codes.  Sums, norms and scales are 32-bit; the only rounding to fewer bits is the code itself.
+// kvad_int8_read: codes back to numbers.
+#include "common.cuh"
+
+using namespace kvad;
+
+KVAD_DEFINE_LAST_ERROR()
+
+namespace {
+
+enum Norm : int { NORM_NONE = 0, NORM_RMS = 1, NORM_LAYER = 2 };
+
+// Four consecutive entries as floats.
+__device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 load4(const __nv_bfloat16* p) {
+  const uint2 q = *reinterpret_cast<const uint2*>(p);
+  return make_float4(__uint_as_float(q.x << 16), __uint_as_float(q.x & 0xffff0000u), __uint_as_float(q.y << 16), __uint_as_float(q.y & 0xffff0000u));
+}
+__device__ __forceinline__ float4 load4_param(const void* p, int64_t i, int is_f32) {
+  return is_f32 ? load4(reinterpret_cast<const float*>(p) + i) : load4(reinterpret_cast<const __nv_bfloat16*>(p) + i);
+}
+__device__ __forceinline__ void store4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
+__device__ __forceinline__ void store4(__nv_bfloat16* p, float4 v) {
+  __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+  *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
+}
+
+// Sum / maximum over the threads of one row: TPR of them, whole warps of one block (several rows a block only where TPR is a warp).
+template <int TPR> __device__ __forceinline__ float row_sum(float v, float* scratch) {
+  v = warp_sum(v);
+  if (TPR == 32) return v;
+  __syncthreads();                          // (the scratch of the reduction before has been read)
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float t = 0.f;
+#pragma unroll
+  for (int i = 0; i < TPR / 32; ++i) t += scratch[i];
+  return t;
+}
+template <int TPR> __device__ __forceinline__ uint32_t row_max(uint32_t v, float* scratch) {
+  v = __reduce_max_sync(0xffffffffu, v);
+  if (TPR == 32) return v;
+  uint32_t* s = reinterpret_cast<uint32_t*>(scratch);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+  __syncthreads();
+  uint32_t t = 0;
+#pragma unroll
+  for (int i = 0; i < TPR / 32; ++i) t = s[i] > t ? s[i] : t;
+  return t;
+}
+
+// TPR threads a row, 4 * V entries a thread at most.  VEC: four entries at a time (every row on a 4-entry boundary), else one.
+template <typename T, int NORM, int TPR, int V, bool VEC>
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
+int8_rows_kernel(const T* __restrict__ x, int64_t ld_x, const int* __restrict__ rows, const void* __restrict__ delta, int delta_f32, int64_t ld_delta,
+                 float mult, float* __restrict__ x_out, int64_t ld_out, const void* __restrict__ weight, const void* __restrict__ bias, int params_f32,
+                 int unit_offset, int8_t* __restrict__ codes, int64_t ld_codes, float* __restrict__ scales, int n, int width, float eps) {
+  constexpr int BLOCK = TPR < 128 ? 128 : TPR;
+  __shared__ float scratch[TPR == 32 ? 1 : TPR / 32];
+  pdl_launch_dependents();
+  const int t = threadIdx.x % TPR;
+  const int64_t r = (int64_t)blockIdx.x * (BLOCK / TPR) + threadIdx.x / TPR;
+  // entry e of this thread's: four together (VEC) or one, dealt out so that neighbours' entries are neighbours
+  auto place = [&](int e) { return VEC ? ((e >> 2) * TPR + t) * 4 + (e & 3) : e * TPR + t; };
+  pdl_wait();
+  if (r >= n) return;                       // (only where a row is a warp's: no barrier follows)
+  const int64_t src = rows != nullptr ? rows[r] : r;
+  const T* xr = x + src * ld_x;
+  float v[4 * V];
+#pragma unroll
+  for (int e = 0; e < 4 * V; e += VEC ? 4 : 1) {
+    const int j = place(e);
+    if (VEC) {
+      const float4 q = j < width ? load4(xr + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+      v[e] = q.x; v[e + 1] = q.y; v[e + 2] = q.z; v[e + 3] = q.w;
+    } else {
+      v[e] = j < width ? to_f32(xr[j]) : 0.f;
+    }
+  }
+  if (NORM != NORM_NONE) {
+    if (delta != nullptr) {
+#pragma unroll
+      for (int e = 0; e < 4 * V; e += VEC ? 4 : 1) {
+        const int j = place(e);
+        if (j < width) {
+          if (VEC) {
+            const float4 d = load4_param(delta, src * ld_delta + j, delta_f32);
+            v[e] = fmaf(mult, d.x, v[e]); v[e + 1] = fmaf(mult, d.y, v[e + 1]); v[e + 2] = fmaf(mult, d.z, v[e + 2]); v[e + 3] = fmaf(mult, d.w, v[e + 3]);
+          } else {
+            v[e] = fmaf(mult, load_param(delta, src * ld_delta + j, delta_f32), v[e]);
+          }
+        }
+      }
+    }
+    if (x_out != nullptr) {
+#pragma unroll
+      for (int e = 0; e < 4 * V; e += VEC ? 4 : 1) {
+        const int j = place(e);
+        if (j < width) {
+          if (VEC) store4(x_out + src * ld_out + j, make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]));
+          else x_out[src * ld_out + j] = v[e];
+        }
+      }
+    }
+    const float inv_width = 1.f / (float)width;
+    if (NORM == NORM_LAYER) {
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4 * V; ++e) sum += v[e];
+      const float mean = row_sum<TPR>(sum, scratch) * inv_width;
+#pragma unroll
+      for (int e = 0; e < 4 * V; ++e) v[e] = place(e) < width ? v[e] - mean : 0.f;
+    }
+    float sq = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4 * V; ++e) sq = fmaf(v[e], v[e], sq);
+    const float rstd = 1.f / sqrtf(row_sum<TPR>(sq, scratch) * inv_width + eps);
+#pragma unroll
+    for (int e = 0; e < 4 * V; e += VEC ? 4 : 1) {
+      const int j = place(e);
+      if (j < width) {
+        if (VEC) {
+          float4 w = make_float4(1.f, 1.f, 1.f, 1.f), b = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (weight != nullptr) w = load4_param(weight, j, params_f32);
+          if (bias != nullptr) b = load4_param(bias, j, params_f32);
+          const float one = unit_offset ? 1.f : 0.f;
+          v[e] = fmaf(v[e] * rstd, w.x + one, b.x); v[e + 1] = fmaf(v[e + 1] * rstd, w.y + one, b.y);
+          v[e + 2] = fmaf(v[e + 2] * rstd, w.z + one, b.z); v[e + 3] = fmaf(v[e + 3] * rstd, w.w + one, b.w);
+        } else {
+          const float w = (weight != nullptr ? load_param(weight, j, params_f32) : 1.f) + (unit_offset ? 1.f : 0.f);
+          v[e] = fmaf(v[e] * rstd, w, bias != nullptr ? load_param(bias, j, params_f32) : 0.f);
+        }
+      }
+    }
+  }
+  uint32_t top = 0;                          // largest magnitude, as bits: NaN and infinity are above every finite number
+#pragma unroll
+  for (int e = 0; e < 4 * V; ++e) {
+    const uint32_t bits = __float_as_uint(v[e]) & 0x7fffffffu;
+    top = bits > top ? bits : top;
+  }
+  top = row_max<TPR>(top, scratch);
+  const bool finite = top < 0x7f800000u;
+  const float scale = finite ? __fmul_rn(__uint_as_float(top), 1.f / 127.f) : __uint_as_float(0x7fffffffu);
+  const bool some = finite && scale > 0.f;
+  if (t == 0) scales[r] = scale;
+  int8_t* cr = codes + r * ld_codes;
+#pragma unroll
+  for (int e = 0; e < 4 * V; e += VEC ? 4 : 1) {
+    const int j = place(e);
+    if (j < width) {
+      int c[4];
+#pragma unroll
+      for (int i = 0; i < (VEC ? 4 : 1); ++i) {
+        // (a scale below the smallest normal number is off by up to half: the quotient may then pass 127)
+        const float q = some ? __fdiv_rn(v[e + i], scale) : 0.f;
+        c[i] = __float2int_rn(fminf(fmaxf(q, -127.f), 127.f));
+      }
+      if (VEC) *reinterpret_cast<uint32_t*>(cr + j) = (c[0] & 0xff) | (c[1] & 0xff) << 8 | (c[2] & 0xff) << 16 | (uint32_t)(c[3] & 0xff) << 24;
+      else cr[j] = (int8_t)c[0];
+    }
+  }
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256)
+int8_read_kernel(const int8_t* __restrict__ codes, int64_t ld_codes, const float* __restrict__ scales, T* __restrict__ out, int64_t ld_out, int n, int width) {
+  pdl_launch_dependents();
+  const int per_row = VEC ? (width + 15) / 16 : width;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  pdl_wait();
+  if (i >= (int64_t)n * per_row) return;
+  const int64_t r = i / per_row;
+  const int j = (int)(i - r * per_row) * (VEC ? 16 : 1);
+  const float s = scales[r];
+  if (VEC) {
+    const int4 q = *reinterpret_cast<const int4*>(codes + r * ld_codes + j);
+    const int w[4] = {q.x, q.y, q.z, q.w};
+    T* o = out + r * ld_out + j;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      store4(o + 4 * k, make_float4((float)(int8_t)w[k] * s, (float)(int8_t)(w[k] >> 8) * s, (float)(int8_t)(w[k] >> 16) * s, (float)(w[k] >> 24) * s));
+  } else {
+    out[r * ld_out + j] = from_f32<T>((float)codes[r * ld_codes + j] * s);
+  }
+}
+
+bool aligned(const void* p, int64_t ld, int entry, int entries) {
+  return p == nullptr || (reinterpret_cast<uintptr_t>(p) % (entry * entries) == 0 && ld % entries == 0);
+}
+
+struct Call {
+  const void* x; int64_t ld_x; const int* rows; const void* delta; int delta_f32; int64_t ld_delta; float mult; float* x_out; int64_t ld_out;
+  const void* weight; const void* bias; int params_f32, unit_offset; int8_t* codes; int64_t ld_codes; float* scales; int n, width; float eps;
+  cudaStream_t stream;
+};
+
+template <typename T, int NORM, int TPR, int V, bool VEC> cudaError_t go(const Call& c) {
+  constexpr int BLOCK = TPR < 128 ? 128 : TPR;
+  const int per_block = BLOCK / TPR;
+  return kvad_launch(int8_rows_kernel<T, NORM, TPR, V, VEC>, dim3((unsigned)((c.n + per_block - 1) / per_block)), dim3(BLOCK), 0, c.stream,
+                     reinterpret_cast<const T*>(c.x), c.ld_x, c.rows, c.delta, c.delta_f32, c.ld_delta, c.mult, c.x_out, c.ld_out, c.weight, c.bias,
+                     c.params_f32, c.unit_offset, c.codes, c.ld_codes, c.scales, c.n, c.width, c.eps);
+}
+
+// Threads for a row: a warp up to 512 entries, then as many as give each 16 entries, then 32.
+template <typename T, int NORM, bool VEC> cudaError_t by_width(const Call& c) {
+  if (c.width <= 128) return go<T, NORM, 32, 1, VEC>(c);
+  if (c.width <= 512) return go<T, NORM, 32, 4, VEC>(c);
+  if (c.width <= 2048) return go<T, NORM, 128, 4, VEC>(c);
+  if (c.width <= 4096) return go<T, NORM, 256, 4, VEC>(c);
+  if (c.width <= 8192) return go<T, NORM, 512, 4, VEC>(c);
+  if (c.width <= 16384) return go<T, NORM, 1024, 4, VEC>(c);
+  return go<T, NORM, 1024, 8, VEC>(c);
+}
+
+}  // namespace
+
+KVAD_EXPORT int kvad_int8_rows(int dtype, int norm, const void* x, int64_t ld_x, const int* rows, const void* delta, int delta_f32, int64_t ld_delta,
+                               float mult, float* x_out, int64_t ld_out, const void* weight, const void* bias, int params_f32, int unit_offset,
+                               int8_t* codes, int64_t ld_codes, float* scales, int n, int width, float eps, cudaStream_t stream) {
+  KVAD_REQUIRE(n > 0 && width > 0, "int8_rows: needs rows, got %d of %d entries", n, width);
+  if (width > 32768) KVAD_FAIL(KVAD_ERR_UNSUPPORTED, "int8_rows: rows of at most 32768 entries, got %d", width);
+  KVAD_REQUIRE(norm >= NORM_NONE && norm <= NORM_LAYER, "int8_rows: unknown norm %d", norm);
+  KVAD_REQUIRE(norm == NORM_NONE || dtype == KVAD_DTYPE_F32, "int8_rows: norms read the float32 stream");
+  KVAD_REQUIRE(norm != NORM_NONE || (delta == nullptr && x_out == nullptr && weight == nullptr && bias == nullptr), "int8_rows: sums and weights go with a norm");
+  const Call c{x, ld_x, rows, delta, delta_f32, ld_delta, mult, x_out, ld_out, weight, bias, params_f32, unit_offset, codes, ld_codes, scales, n, width, eps, stream};
+  const int size = dtype == KVAD_DTYPE_F32 ? 4 : 2, p_size = params_f32 ? 4 : 2;
+  const bool vec = width % 4 == 0 && aligned(x, ld_x, size, 4) && aligned(delta, ld_delta, delta_f32 ? 4 : 2, 4) && aligned(x_out, ld_out, 4, 4) &&
+                   aligned(weight, 0, p_size, 4) && aligned(bias, 0, p_size, 4) && aligned(codes, ld_codes, 1, 4);
+  cudaError_t e;
+  if (norm == NORM_RMS) e = vec ? by_width<float, NORM_RMS, true>(c) : by_width<float, NORM_RMS, false>(c);
+  else if (norm == NORM_LAYER) e = vec ? by_width<float, NORM_LAYER, true>(c) : by_width<float, NORM_LAYER, false>(c);
+  else if (dtype == KVAD_DTYPE_F32) e = vec ? by_width<float, NORM_NONE, true>(c) : by_width<float, NORM_NONE, false>(c);
+  else e = vec ? by_width<__nv_bfloat16, NORM_NONE, true>(c) : by_width<__nv_bfloat16, NORM_NONE, false>(c);
+  if (e != cudaSuccess) KVAD_FAIL(KVAD_ERR_CUDA, "int8_rows: launch failed: %s", cudaGetErrorString(e));
+  KVAD_CHECK_LAUNCH("int8_rows");
+  return KVAD_OK;
+}
+
+KVAD_EXPORT int kvad_int8_read(int dtype, const int8_t* codes, int64_t ld_codes, const float* scales, void* out, int64_t ld_out, int n, int width,
+                               cudaStream_t stream) {
+  KVAD_REQUIRE(n > 0 && width > 0, "int8_read: needs rows, got %d of %d entries", n, width);
+  const bool f32 = dtype == KVAD_DTYPE_F32;
+  const bool vec = width % 16 == 0 && aligned(codes, ld_codes, 1, 16) && aligned(out, ld_out, f32 ? 4 : 2, 4);
+  const int64_t pieces = (int64_t)n * (vec ? width / 16 : width), blocks = (pieces + 255) / 256;
+  KVAD_REQUIRE(blocks < (1ll << 31), "int8_read: %d rows of %d entries are more than a launch takes", n, width);
+  cudaError_t e;
+  auto launch = [&](auto kernel, auto* o) { return kvad_launch(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, codes, ld_codes, scales, o, ld_out, n, width); };
+  if (f32) e = vec ? launch(int8_read_kernel<float, true>, (float*)out) : launch(int8_read_kernel<float, false>, (float*)out);
+  else e = vec ? launch(int8_read_kernel<__nv_bfloat16, true>, (__nv_bfloat16*)out) : launch(int8_read_kernel<__nv_bfloat16, false>, (__nv_bfloat16*)out);
+  if (e != cudaSuccess) KVAD_FAIL(KVAD_ERR_CUDA, "int8_read: launch failed: %s", cudaGetErrorString(e));
+  KVAD_CHECK_LAUNCH("int8_read");
+  return KVAD_OK;
+}

@@ -206,6 +206,24 @@ _SIGNATURES = {
         "kvad_streams_norm": [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                               c_int, c_int, c_void_p, c_int, c_int, c_int, c_float, c_void_p],
     },
+    "int8_rows": {
+        "kvad_int8_rows": [c_int, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int64, c_float, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int,
+                           c_void_p, c_int64, c_void_p, c_int, c_int, c_float, c_void_p],
+        "kvad_int8_read": [c_int, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p],
+    },
+    "int8_cache": {
+        "kvad_kv_store_int8": [c_int, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                               c_int, c_int, c_int, c_void_p],
+        "kvad_kv_read_int8": [c_int, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                              c_int, c_int, c_int, c_int, c_void_p],
+    },
+    "linear_int8": {
+        "kvad_linear_int8": [c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_void_p],
+    },
+    "attention_int8": {
+        "kvad_attention_int8": [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                                c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p],
+    },
     "sampling": {
         "kvad_sample": [c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
         "kvad_argmax": [c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p],
@@ -282,6 +300,7 @@ _FAMILY_LIBRARIES = {
     "moe": {"any": ("moe",)},
     "channel_recurrence": {"any": ("channel_recurrence",)},
     "streams": {"any": ("streams",)},
+    "int8": {"any": ("int8_rows", "int8_cache", "linear_int8", "attention_int8")},
 }
 
 
@@ -1765,6 +1784,177 @@ class Ops:
         _check(h.kvad_streams_norm(_code(out.dtype), _ptr(x), total * width if x.dim() == 3 else 0, _ptr(x_out), total * width, _ptr(y), _ptr(mix),
                                    _ptr(share), _ptr(read), _ptr(rows), _ptr(gain), _ptr(bias), 1 if gain.dtype == torch.float32 else 0,
                                    int(bool(centred)), _ptr(out), n, width, int(copies), float(eps), _stream()), h)
+
+    # -- rows, products, cache and attention in 8-bit codes -----------------------------------------
+    #
+    # A row x held in 8 bits is codes c (int8, -127 .. 127) and a float32 scale s = max|x| / 127: x ~ c s, c = x / s rounded to the nearest
+    # integer, halves to the even one.  A row of zeros has the scale 0; a row with a number that is not finite has the scale NaN and codes 0.
+
+    @staticmethod
+    def _int8_rows_check(what: str, codes, scales, n: int, width: int) -> int:
+        if codes.dtype != torch.int8 or codes.shape != (n, width):
+            raise KernelError(f"{what}: codes must be int8 of shape [{n}, {width}]")
+        if scales.dtype != torch.float32 or scales.numel() != n or not scales.is_contiguous():
+            raise KernelError(f"{what}: scales must be contiguous float32, one per row")
+        return _rows_view(codes, f"{what} codes")
+
+    def int8_rows(self, x, codes, scales) -> None:
+        """Rows of activations or weights (float32 or bfloat16) as 8-bit codes and a scale a row."""
+        _need_cuda(x, codes, scales)
+        ld_x = _rows_view(x, "int8_rows input")
+        n, width = x.shape
+        ld_c = self._int8_rows_check("int8_rows", codes, scales, n, width)
+        h = lib("int8_rows")
+        _check(h.kvad_int8_rows(_code(x.dtype), 0, x.data_ptr(), ld_x, None, None, 0, 0, 0.0, None, 0, None, None, 0, 0, codes.data_ptr(), ld_c,
+                                scales.data_ptr(), n, width, 0.0, _stream()), h)
+
+    def _norm_int8(self, what: str, norm: int, x, weight, bias, eps: float, codes, scales, unit_offset: bool, rows, delta, mult: float, x_out) -> None:
+        _need_cuda(x, weight, bias, codes, scales, rows, delta, x_out)
+        ld_x = _rows_view(x, f"{what} input")
+        width = x.shape[1]
+        n = x.shape[0] if rows is None else rows.numel()
+        if x.dtype != torch.float32:
+            raise KernelError(f"{what}: input must be the float32 residual stream")
+        ld_c = self._int8_rows_check(what, codes, scales, n, width)
+        p_f32 = 0
+        for p in (weight, bias):
+            if p is not None:
+                if p.numel() != width or p.dtype not in (torch.float32, torch.bfloat16) or not p.is_contiguous():
+                    raise KernelError(f"{what}: weight and bias must have the row's width, float32 or bfloat16")
+                p_f32 = 1 if p.dtype == torch.float32 else 0
+        if weight is not None and bias is not None and weight.dtype != bias.dtype:
+            raise KernelError(f"{what}: weight and bias must have one dtype")
+        if rows is not None and (rows.dtype != torch.int32 or not rows.is_contiguous() or delta is not None or x_out is not None):
+            raise KernelError(f"{what}: a row list is contiguous int32, and goes without a sum")
+        ld_d = ld_o = d_f32 = 0
+        if delta is not None:
+            ld_d = _rows_view(delta, f"{what} sum")
+            if delta.shape != x.shape or delta.dtype not in (torch.float32, torch.bfloat16):
+                raise KernelError(f"{what}: what is added must have the stream's shape, float32 or bfloat16")
+            d_f32 = 1 if delta.dtype == torch.float32 else 0
+            if x_out is None:
+                x_out = x
+        if x_out is not None:
+            ld_o = _rows_view(x_out, f"{what} stream")
+            if x_out.shape != x.shape or x_out.dtype != torch.float32:
+                raise KernelError(f"{what}: the stream's output must be float32 of its shape")
+        h = lib("int8_rows")
+        _check(h.kvad_int8_rows(F32, norm, x.data_ptr(), ld_x, _ptr(rows), _ptr(delta), d_f32, ld_d, float(mult), _ptr(x_out), ld_o, _ptr(weight), _ptr(bias),
+                                p_f32, int(unit_offset), codes.data_ptr(), ld_c, scales.data_ptr(), n, width, float(eps), _stream()), h)
+
+    def rmsnorm_int8(self, x, weight, eps: float, codes, scales, *, unit_offset: bool = False, rows=None, delta=None, mult: float = 1.0, x_out=None) -> None:
+        """The RMS norm of the float32 stream's rows as 8-bit codes and a scale a row: y = t / sqrt(mean(t^2) + eps) * w (`weight` None: no weight;
+        `unit_offset`: 1 is added to it), t = x + mult * delta where a `delta` (float32 or bfloat16) is given.  The sum t is written to `x_out`, or
+        into x itself.  `rows`: only these rows of x (no sum then)."""
+        self._norm_int8("rmsnorm_int8", 1, x, weight, None, eps, codes, scales, unit_offset, rows, delta, mult, x_out)
+
+    def layernorm_int8(self, x, gain, bias, eps: float, codes, scales, *, rows=None, delta=None, mult: float = 1.0, x_out=None) -> None:
+        """The layer norm of the float32 stream's rows as 8-bit codes and a scale a row; sums and rows as in `rmsnorm_int8`."""
+        self._norm_int8("layernorm_int8", 2, x, gain, bias, eps, codes, scales, False, rows, delta, mult, x_out)
+
+    def int8_read(self, codes, scales, out) -> None:
+        """What rows of codes stand for: out = codes * scale, float32 or bfloat16."""
+        _need_cuda(codes, scales, out)
+        ld_o = _rows_view(out, "int8_read output")
+        n, width = out.shape
+        ld_c = self._int8_rows_check("int8_read", codes, scales, n, width)
+        h = lib("int8_rows")
+        _check(h.kvad_int8_read(_code(out.dtype), codes.data_ptr(), ld_c, scales.data_ptr(), out.data_ptr(), ld_o, n, width, _stream()), h)
+
+    def linear_int8(self, a, a_scales, weight, w_scales, bias, out, epilogue: str = "store") -> None:
+        """out = epilogue((a . weight^T) * a_scales[row] * w_scales[output] + bias): rows and weights ([out_features, in_features]) as 8-bit codes with a
+        scale a row of each; the sums of products are exact whole numbers.  Inputs of a multiple of 16 entries."""
+        _need_cuda(a, a_scales, weight, w_scales, bias, out)
+        epi = EPILOGUES[epilogue]
+        lda, ldo = _rows_view(a, "linear_int8 input"), _rows_view(out, "linear_int8 output")
+        m, k = a.shape
+        n = weight.shape[0]
+        if weight.dim() != 2 or weight.shape[1] != k or not weight.is_contiguous():
+            raise KernelError(f"linear_int8: weight {tuple(weight.shape)} does not take inputs of width {k}")
+        if a.dtype != torch.int8 or weight.dtype != torch.int8:
+            raise KernelError("linear_int8: input and weight must be int8")
+        if (a_scales.dtype != torch.float32 or a_scales.numel() != m or not a_scales.is_contiguous() or w_scales.dtype != torch.float32
+                or w_scales.numel() != n or not w_scales.is_contiguous()):
+            raise KernelError("linear_int8: scales must be contiguous float32, one per row and one per output")
+        want_out = torch.float32 if epi >= 3 else self.dtype
+        if out.dtype != want_out or out.shape[0] != m or out.shape[1] != n:
+            raise KernelError(f"linear_int8: output must be {want_out} of shape [{m}, {n}]")
+        bias_f32 = 0
+        if bias is not None:
+            if bias.numel() != n or bias.dtype not in (torch.float32, torch.bfloat16) or not bias.is_contiguous():
+                raise KernelError(f"linear_int8: the bias must have {n} entries, float32 or bfloat16")
+            bias_f32 = 1 if bias.dtype == torch.float32 else 0
+        h = lib("linear_int8")
+        _check(h.kvad_linear_int8(self.code, a.data_ptr(), lda, a_scales.data_ptr(), weight.data_ptr(), w_scales.data_ptr(), _ptr(bias), bias_f32,
+                                  out.data_ptr(), ldo, m, n, k, epi, _stream()), h)
+
+    @staticmethod
+    def _int8_pages(what: str, k_pages, k_scales, v_pages, v_scales) -> tuple:
+        if k_pages.dim() != 4 or k_pages.dtype != torch.int8 or v_pages.dtype != torch.int8 or v_pages.shape != k_pages.shape \
+                or not k_pages.is_contiguous() or not v_pages.is_contiguous():
+            raise KernelError(f"{what}: pages must be contiguous int8 [pages, kv heads, page size, head size], keys and values alike")
+        cells = k_pages.shape[:3]
+        if k_scales.dtype != torch.float32 or v_scales.dtype != torch.float32 or k_scales.shape != cells or v_scales.shape != cells \
+                or not k_scales.is_contiguous() or not v_scales.is_contiguous():
+            raise KernelError(f"{what}: scales must be contiguous float32 [pages, kv heads, page size]")
+        return k_pages.shape
+
+    def kv_store_int8(self, k_src, v_src, row_seq, row_pos, page_table, k_pages, k_scales, v_pages, v_scales) -> None:
+        """Writes the rows' keys and values (views `[rows, kv_heads * head_dim]` of one buffer) into their sequences' pages as 8-bit codes, with a
+        scale for each position and head.  Head sizes are multiples of 16 up to 256."""
+        _need_cuda(k_src, v_src, row_seq, row_pos, page_table, k_pages, k_scales, v_pages, v_scales)
+        ld = _rows_view(k_src, "new keys")
+        _, n_kv, page, hd = self._int8_pages("kv_store_int8", k_pages, k_scales, v_pages, v_scales)
+        n = k_src.shape[0]
+        if (_rows_view(v_src, "new values") != ld or k_src.shape != (n, n_kv * hd) or v_src.shape != k_src.shape or k_src.dtype != self.dtype
+                or v_src.dtype != self.dtype):
+            raise KernelError(f"kv_store_int8: keys and values must be {self.dtype} views [rows, {n_kv} x {hd}] of one buffer")
+        self._rows_of_pages("kv_store_int8", n, row_seq, row_pos, page_table)
+        h = lib("int8_cache")
+        _check(h.kvad_kv_store_int8(self.code, k_src.data_ptr(), v_src.data_ptr(), ld, row_seq.data_ptr(), row_pos.data_ptr(), page_table.data_ptr(),
+                                    page_table.shape[1], k_pages.data_ptr(), k_scales.data_ptr(), v_pages.data_ptr(), v_scales.data_ptr(), n, n_kv, hd, page,
+                                    _stream()), h)
+
+    @staticmethod
+    def _rows_of_pages(what: str, n: int, row_seq, row_pos, page_table) -> None:
+        if (row_seq.dtype != torch.int32 or row_pos.dtype != torch.int32 or row_seq.numel() < n or row_pos.numel() < n or page_table.dtype != torch.int32
+                or page_table.dim() != 2 or not page_table.is_contiguous()):
+            raise KernelError(f"{what}: the rows' sequences and positions are int32, one per row, and the page table a contiguous int32 matrix")
+
+    def kv_read_int8(self, row_seq, row_pos, page_table, k_pages, k_scales, v_pages, v_scales, k_out, v_out) -> None:
+        """What the cache holds for the rows: k_out, v_out `[rows, kv_heads * head_dim]` = codes * scale of each row's sequence and position."""
+        _need_cuda(row_seq, row_pos, page_table, k_pages, k_scales, v_pages, v_scales, k_out, v_out)
+        _, n_kv, page, hd = self._int8_pages("kv_read_int8", k_pages, k_scales, v_pages, v_scales)
+        n = k_out.shape[0]
+        ld_k, ld_v = _rows_view(k_out, "keys read"), _rows_view(v_out, "values read")
+        if k_out.shape != (n, n_kv * hd) or v_out.shape != k_out.shape or k_out.dtype != self.dtype or v_out.dtype != self.dtype:
+            raise KernelError(f"kv_read_int8: keys and values must be {self.dtype} [rows, {n_kv} x {hd}]")
+        self._rows_of_pages("kv_read_int8", n, row_seq, row_pos, page_table)
+        h = lib("int8_cache")
+        _check(h.kvad_kv_read_int8(self.code, k_out.data_ptr(), v_out.data_ptr(), ld_k, ld_v, row_seq.data_ptr(), row_pos.data_ptr(), page_table.data_ptr(),
+                                   page_table.shape[1], k_pages.data_ptr(), k_scales.data_ptr(), v_pages.data_ptr(), v_scales.data_ptr(), n, n_kv, hd, page,
+                                   _stream()), h)
+
+    def attention_int8(self, q, out, seq_starts, kv_lens, n_seqs: int, max_new: int, page_table, k_pages, k_scales, v_pages, v_scales, n_heads: int,
+                       scale: float, *, window: int = 0, keep_first: int = 0) -> None:
+        """Causal softmax attention of packed rows (each sequence's rows are its last positions; `max_new`: the longest run of them) over the paged cache
+        of 8-bit codes (`kv_store_int8`).  A row sees the positions up to its own, or with a `window` the last so many and always the first
+        `keep_first`.  Several query heads may share a key/value head.  Head sizes are multiples of 16 up to 256, pages hold 64 positions."""
+        _need_cuda(q, out, seq_starts, kv_lens, page_table, k_pages, k_scales, v_pages, v_scales)
+        ld_q, ld_o = _rows_view(q, "attention queries"), _rows_view(out, "attention output")
+        _, n_kv, page, hd = self._int8_pages("attention_int8", k_pages, k_scales, v_pages, v_scales)
+        n = q.shape[0]
+        if q.shape[1] != n_heads * hd or out.shape != q.shape:
+            raise KernelError("attention_int8: queries/output do not match heads x head size")
+        if q.dtype != self.dtype or out.dtype != self.dtype:
+            raise KernelError(f"attention_int8: queries and output must be {self.dtype}")
+        if (seq_starts.dtype != torch.int32 or kv_lens.dtype != torch.int32 or seq_starts.numel() <= n_seqs or kv_lens.numel() < n_seqs
+                or page_table.dtype != torch.int32 or page_table.dim() != 2 or not page_table.is_contiguous() or page_table.shape[0] < n_seqs):
+            raise KernelError("attention_int8: starts, lengths and the page table are int32, an entry (and one start more) per sequence")
+        h = lib("attention_int8")
+        _check(h.kvad_attention_int8(self.code, q.data_ptr(), ld_q, out.data_ptr(), ld_o, seq_starts.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(),
+                                     page_table.shape[1], k_pages.data_ptr(), k_scales.data_ptr(), v_pages.data_ptr(), v_scales.data_ptr(), n, int(n_seqs),
+                                     int(max_new), int(n_heads), n_kv, hd, page, float(scale), int(window or 0), int(keep_first or 0), _stream()), h)
 
     # -- sampling ------------------------------------------------------------------
     ARGMAX_CHUNK = 2048
