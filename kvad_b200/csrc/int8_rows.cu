@@ -70,7 +70,8 @@ int8_rows_kernel(const T* __restrict__ x, int64_t ld_x, const int* __restrict__ 
                  int unit_offset, int8_t* __restrict__ codes, int64_t ld_codes, float* __restrict__ scales, int n, int width, float eps) {
   constexpr int BLOCK = TPR < 128 ? 128 : TPR;
   __shared__ float scratch[TPR == 32 ? 1 : TPR / 32];
-  pdl_launch_dependents();
+  // (what rows without a norm become may be weights, which the products fetch before they wait for the kernel before them: no early start there)
+  if (NORM != NORM_NONE) pdl_launch_dependents();
   const int t = threadIdx.x % TPR;
   const int64_t r = (int64_t)blockIdx.x * (BLOCK / TPR) + threadIdx.x / TPR;
   // entry e of this thread's: four together (VEC) or one, dealt out so that neighbours' entries are neighbours

@@ -218,7 +218,9 @@ _SIGNATURES = {
                               c_int, c_int, c_int, c_int, c_void_p],
     },
     "linear_int8": {
-        "kvad_linear_int8": [c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_void_p],
+        "kvad_linear_int8": [c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_void_p],
+        "kvad_linear_int8_status": [],
+        "kvad_linear_int8_test_hooks": [c_uint, c_int],
     },
     "attention_int8": {
         "kvad_attention_int8": [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -1861,9 +1863,10 @@ class Ops:
         h = lib("int8_rows")
         _check(h.kvad_int8_read(_code(out.dtype), codes.data_ptr(), ld_c, scales.data_ptr(), out.data_ptr(), ld_o, n, width, _stream()), h)
 
-    def linear_int8(self, a, a_scales, weight, w_scales, bias, out, epilogue: str = "store") -> None:
+    def linear_int8(self, a, a_scales, weight, w_scales, bias, out, epilogue: str = "store", *, form: int = 0) -> None:
         """out = epilogue((a . weight^T) * a_scales[row] * w_scales[output] + bias): rows and weights ([out_features, in_features]) as 8-bit codes with a
-        scale a row of each; the sums of products are exact whole numbers.  Inputs of a multiple of 16 entries."""
+        scale a row of each; the sums of products are exact whole numbers.  Inputs of a multiple of 16 entries.  `form`: 0: chosen by the sizes; 1: weights
+        streamed (at most 64 rows); 64, 128, 256: the tensor-core kernel with tiles so wide."""
         _need_cuda(a, a_scales, weight, w_scales, bias, out)
         epi = EPILOGUES[epilogue]
         lda, ldo = _rows_view(a, "linear_int8 input"), _rows_view(out, "linear_int8 output")
@@ -1886,7 +1889,7 @@ class Ops:
             bias_f32 = 1 if bias.dtype == torch.float32 else 0
         h = lib("linear_int8")
         _check(h.kvad_linear_int8(self.code, a.data_ptr(), lda, a_scales.data_ptr(), weight.data_ptr(), w_scales.data_ptr(), _ptr(bias), bias_f32,
-                                  out.data_ptr(), ldo, m, n, k, epi, _stream()), h)
+                                  out.data_ptr(), ldo, m, n, k, epi, int(form), _stream()), h)
 
     @staticmethod
     def _int8_pages(what: str, k_pages, k_scales, v_pages, v_scales) -> tuple:
@@ -2125,6 +2128,11 @@ def scored_wide_wait_timeouts() -> int:
     if n < 0:
         raise KernelError(h.kvad_last_error().decode("utf-8", "replace"))
     return n
+
+
+def linear_int8_wait_timeouts() -> int:
+    """How many bounded waits of the products of 8-bit rows have run out in this process (0 unless something is wrong).  Synchronises the device."""
+    return int(lib("linear_int8").kvad_linear_int8_status())
 
 
 def scored_prompt_wait_timeouts() -> int:

@@ -144,7 +144,7 @@ def gelu(y, form):
     return y / (1 + torch.exp(-2 * 0.79788456 * (y + 0.044715 * y ** 3)))
 
 
-def check_product(dtype, m, n, k, epilogue, bias=True, extra=0):
+def check_product(dtype, m, n, k, epilogue, bias=True, extra=0, form=0):
     a, sa, w, sw, b = product(m + n + k, m, n, k, extra)
     b = b if bias is True else None if not bias else b.to(DT[bias])
     whole = (a.double() @ w.double().T)                      # exact: every sum is below 2^53
@@ -152,7 +152,7 @@ def check_product(dtype, m, n, k, epilogue, bias=True, extra=0):
     out_dtype = torch.float32 if epilogue in ("residual", "store_f32") else DT[dtype]
     base = torch.randn(m, n, device="cuda", generator=generator(5)) if epilogue == "residual" else torch.full((m, n), float("nan"), device="cuda")
     out = apart(base.to(out_dtype), 5) if extra else base.to(out_dtype).clone()
-    Ops(DT[dtype]).linear_int8(a, sa, w, sw, b, out, epilogue)
+    Ops(DT[dtype]).linear_int8(a, sa, w, sw, b, out, epilogue, form=form)
     # the sum's own rounding to 32 bits, the two scales', the bias'
     off = 4 * 2.0 ** -24 * ((y - (0 if b is None else b.double())).abs() + y.abs())
     if epilogue == "residual":
@@ -173,6 +173,14 @@ def check_product(dtype, m, n, k, epilogue, bias=True, extra=0):
                                             ("bfloat16", "store_f32")])
 def test_products(m, n, k, dtype, epilogue):
     check_product(dtype, m, n, k, epilogue)
+
+
+# every form on its own: tiles of rows and outputs in part, more tiles than SMs, K of one block and of many
+@pytest.mark.parametrize("form,m,n,k", [(1, 1, 40, 32), (1, 50, 70, 1616), (64, 1, 100, 16), (64, 300, 9000, 144), (128, 40, 129, 256), (128, 500, 6000, 128), (256, 3, 3, 1040),
+                                        (256, 1100, 5000, 272), (256, 2500, 4800, 400)])
+@pytest.mark.parametrize("dtype,epilogue", [("bfloat16", "store"), ("float32", "store"), ("bfloat16", "residual")])
+def test_products_by_form(form, m, n, k, dtype, epilogue):
+    check_product(dtype, m, n, k, epilogue, form=form)
 
 
 @pytest.mark.parametrize("m", [1, 9, 40, 150])
