@@ -226,6 +226,12 @@ _SIGNATURES = {
         "kvad_attention_int8": [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                 c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p],
     },
+    "attention_int8_prompt": {
+        "kvad_attention_int8_prompt": [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                                       c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p],
+        "kvad_attention_int8_prompt_status": [],
+        "kvad_attention_int8_prompt_test_hooks": [c_uint, c_int],
+    },
     "sampling": {
         "kvad_sample": [c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
         "kvad_argmax": [c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p],
@@ -302,7 +308,7 @@ _FAMILY_LIBRARIES = {
     "moe": {"any": ("moe",)},
     "channel_recurrence": {"any": ("channel_recurrence",)},
     "streams": {"any": ("streams",)},
-    "int8": {"any": ("int8_rows", "int8_cache", "linear_int8", "attention_int8")},
+    "int8": {"any": ("int8_rows", "int8_cache", "linear_int8", "attention_int8"), torch.bfloat16: ("attention_int8_prompt",)},
 }
 
 
@@ -1938,6 +1944,8 @@ class Ops:
                                    page_table.shape[1], k_pages.data_ptr(), k_scales.data_ptr(), v_pages.data_ptr(), v_scales.data_ptr(), n, n_kv, hd, page,
                                    _stream()), h)
 
+    INT8_PROMPT_HEAD_SIZES = (64, 128)
+
     def attention_int8(self, q, out, seq_starts, kv_lens, n_seqs: int, max_new: int, page_table, k_pages, k_scales, v_pages, v_scales, n_heads: int,
                        scale: float, *, window: int = 0, keep_first: int = 0) -> None:
         """Causal softmax attention of packed rows (each sequence's rows are its last positions; `max_new`: the longest run of them) over the paged cache
@@ -1954,6 +1962,15 @@ class Ops:
         if (seq_starts.dtype != torch.int32 or kv_lens.dtype != torch.int32 or seq_starts.numel() <= n_seqs or kv_lens.numel() < n_seqs
                 or page_table.dtype != torch.int32 or page_table.dim() != 2 or not page_table.is_contiguous() or page_table.shape[0] < n_seqs):
             raise KernelError("attention_int8: starts, lengths and the page table are int32, an entry (and one start more) per sequence")
+        if (max_new > 1 and self.dtype == torch.bfloat16 and hd in self.INT8_PROMPT_HEAD_SIZES and page == 64 and n_heads % n_kv == 0 and n_heads // n_kv <= 128
+                and ld_q % 8 == 0 and ld_o % 8 == 0
+                and (q.data_ptr() | out.data_ptr() | k_pages.data_ptr() | v_pages.data_ptr() | k_scales.data_ptr() | v_scales.data_ptr()) % 16 == 0):
+            h = lib("attention_int8_prompt")
+            _check(h.kvad_attention_int8_prompt(q.data_ptr(), ld_q, out.data_ptr(), ld_o, seq_starts.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(),
+                                                page_table.shape[1], k_pages.data_ptr(), k_scales.data_ptr(), v_pages.data_ptr(), v_scales.data_ptr(), n,
+                                                int(n_seqs), int(max_new), int(n_heads), n_kv, hd, page, float(scale), int(window or 0), int(keep_first or 0),
+                                                _stream()), h)
+            return
         h = lib("attention_int8")
         _check(h.kvad_attention_int8(self.code, q.data_ptr(), ld_q, out.data_ptr(), ld_o, seq_starts.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(),
                                      page_table.shape[1], k_pages.data_ptr(), k_scales.data_ptr(), v_pages.data_ptr(), v_scales.data_ptr(), n, int(n_seqs),
@@ -2133,6 +2150,11 @@ def scored_wide_wait_timeouts() -> int:
 def linear_int8_wait_timeouts() -> int:
     """How many bounded waits of the products of 8-bit rows have run out in this process (0 unless something is wrong).  Synchronises the device."""
     return int(lib("linear_int8").kvad_linear_int8_status())
+
+
+def attention_int8_wait_timeouts() -> int:
+    """How many bounded waits of the prompt attention over 8-bit caches have run out in this process (0 unless something is wrong).  Synchronises the device."""
+    return int(lib("attention_int8_prompt").kvad_attention_int8_prompt_status())
 
 
 def scored_prompt_wait_timeouts() -> int:
