@@ -1,24 +1,30 @@
-// Causal attention of prompt rows over the paged cache of 8-bit codes, on the 5th-generation tensor cores (bfloat16, heads of up to 128 entries).
+// Causal attention of prompt rows over the paged cache of 8-bit codes, on the 5th-generation tensor cores (bfloat16 rows, heads of up to 128 entries).
 //
-//   t_ij = log2(e) scale ks_j (q_i . kc_j) + log2(vs_j),    p_ij = 2^(t_ij - m_i),    out_i = sum_j p_ij vc_j / sum_j p_ij / vs_j
+//   t_ij = log2(e) scale q_i . (kc_j ks_j),    out_i = sum_j 2^(t_ij - m_i) vc_j vs_j / sum_j 2^(t_ij - m_i)
 //
-// with kc, vc the codes of key and value j and ks, vs their scales: p is the softmax's weight times the value's scale.  Codes are whole numbers of -127 .. 127, which
-// bfloat16 holds exactly, so both products take the codes as they are and the scales come in as three numbers a key, one multiply-add on the score and one in the sum.
-// What is rounded to bfloat16 is p, as the second product's operand, and the output; scores, maxima, sums and outputs are 32-bit.  With the value's scale inside the exponent the
-// largest p of a row is a power of two, so that a row that attends to one key has that key's value as it is kept.  (A value's scale below 2^-100 counts as 2^-100:
-// weights of keys whose scales are less than 2^100 apart stay within 32-bit numbers.)
+// with kc, vc the codes of key and value j and ks, vs their scales.  Both products run on half-precision operands, whose 11 bits hold a code exactly and make a scaled one, a
+// query or a weight eight times as exact as bfloat16 would.  Their range is small, so powers of two are kept apart:
+//   queries   q_i = 2^a_i q'_i, |q'_i| in [1, 4) at most (bfloat16's 8 bits fit: exact, but for entries below 2^-24 of the row's largest)
+//   keys      log2(e) scale kc ks = 2^(b - 8) k', b the page's largest exponent of a scale; a key's scale in two pieces (22 bits), k' rounded once, an entry at a time
+//   values    vc vs = 2^(c - 8) v', c the page's largest exponent; the scale in one piece
+//   weights   p_ij = 2^(t_ij + c - r_i + 6), r_i the largest t + c seen, or up to 8 less: what is small beside it loses bits below 2^-20 of it
+// so that what a thread does to a score is one multiply-add (by 2^(a + b - 8), plus c - r + 6) and one exponential, and nothing is fetched for each key: scales a
+// key, broadcast from shared memory to a row's thread, held the kernel up before (a wavefront a number: 3 x 128 x 8 warps a step beside the products' own reads).
+// Scores, maxima, sums and outputs are 32-bit.
 //
 // A block has two SLOTS of 128 rows: rows are (token, head) pairs of one key/value head's group, so that the heads that share keys share the work of bringing them.
 // Keys come in steps of two pages (128).  Roles, by warp:
 //   0       brings the queries by TMA and the pages' codes and scales, as they lie, by bulk copies into a ring
 //   1, 2    issue the products of a slot each:  S = Q K^T (128 x 128), then T += P V with P in tensor memory, over S's own columns
-//   4-7     turn codes to bfloat16 in the layout the products read (128-byte swizzle): two shifts of bytes to a place, two masks and one subtraction for two
-//           entries, once for both slots' 256 rows
+//   4-7     turn codes to half precision in the layout the products read (128-byte swizzle), once for both slots' 256 rows: a code's byte under 0x64 is 1024 + code + 128
 //   8-11, 12-15  a thread a row: scores to weights.  The running output stays in tensor memory; it is scaled down only when a row's maximum has risen by
-//           more than 2^8 since the last time (weights are then at most 2^8, and as exact as any), which after the first steps is hardly ever
+//           more than 2^8 since the last time, which after the first steps is hardly ever
 //
-// Keys a row does not see weigh nothing; what a page holds beyond the sequence's end are some codes, which are finite, with scales that are not looked at.
+// Keys a row does not see weigh nothing; scales beyond the sequence's end are taken for zero, whatever they are.  A value whose scale is not finite is a value of zeros for the
+// product, and its key's weight not a number to those rows that see it (such pages take the path that looks at every key).
 // Every wait is bounded; one that runs out raises a counter and the block frees its tensor memory and returns without writing.
+#include <cuda_fp16.h>
+
 #include "scored_tiles.cuh"
 
 using namespace kvad;
@@ -29,9 +35,10 @@ namespace {
 
 constexpr int KEYS = 128;                       // of a step: two pages
 constexpr int THREADS = 512;
-constexpr int REGS_FEW = 56, REGS_TURN = 88, REGS_MANY = 184;       // of 128 a thread at launch: 56 + 88 + 2 * 184 = 4 * 128
+constexpr int REGS_FEW = 72, REGS_TURN = 104, REGS_MANY = 168;      // of 128 a thread at launch: 72 + 104 + 2 * 168 = 4 * 128
 constexpr int SCALE_SETS = 4;
-constexpr float RISE = 8.f, LEAST = 0x1p-100f;
+constexpr float RISE = 8.f, HEAD = 6.f;      // weights are at most 2^(RISE + HEAD)
+constexpr float SHIFT = 256.f;                  // largest scaled code: below 127 * 2 * 2^8, under half precision's 65504
 
 bool g_skip_copy = false;                       // tests: the next launch's blocks leave out their first page
 
@@ -51,14 +58,15 @@ struct Args {
 };
 
 template <int HD> struct Layout {
-  static constexpr int BLOCKS = (HD + 63) / 64;                  // of 64 entries: 128 bytes of bfloat16
-  static constexpr int RING = HD > 64 ? 3 : 6, RAW = 6;         // keys or values of a step as bfloat16; of a page as they came
+  static constexpr int BLOCKS = (HD + 63) / 64;                  // of 64 entries: 128 bytes
+  static constexpr int RING = HD > 64 ? 3 : 6, RAW = 6;         // keys or values of a step in half precision; of a page as they came
   static constexpr uint32_t BLOCK = 128 * 128;                   // 128 rows (or keys) of a block of entries
   static constexpr uint32_t Q_BYTES = BLOCKS * BLOCK, KV_BYTES = BLOCKS * BLOCK;
   static constexpr uint32_t CODES = PAGE * HD, RAW_BYTES = CODES + 2 * PAGE * 4;
+  static constexpr uint32_t SET = 32 + KEYS * 4;                 // of a step: what softmax threads need of its two pages, and marks of its keys
   static constexpr uint32_t OFF_KV = 2 * Q_BYTES, OFF_RAW = OFF_KV + RING * KV_BYTES, OFF_SC = OFF_RAW + RAW * RAW_BYTES;
-  static constexpr uint32_t OFF_BAR = OFF_SC + SCALE_SETS * 3 * KEYS * 4;
-  static constexpr int BARS = 1 + 2 * RING + 2 * RAW + 2 * 3;
+  static constexpr uint32_t OFF_BAR = OFF_SC + SCALE_SETS * SET;
+  static constexpr int BARS = 1 + 2 * RING + 2 * RAW + 2 * 4;
   static constexpr size_t SMEM = OFF_BAR + BARS * 8 + 16 + 1024;
   static constexpr uint32_t TM_O = 2 * KEYS;                     // S (and P) of slot t at t * 128, its output at TM_O + t * 128
   static_assert(SMEM <= 227 * 1024, "an SM's shared memory");
@@ -84,12 +92,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ void scale_pair(uint32_t* x, uint64_t f, uint64_t g) {
-  float u, v;
-  halves(fma2(pair(__uint_as_float(x[0]), __uint_as_float(x[1])), f, g), u, v);
-  x[0] = __float_as_uint(u);
-  x[1] = __float_as_uint(v);
-}
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -100,12 +102,29 @@ __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// Two codes, in bytes 0 and 2 of x, as bfloat16: 0x4300 is 128 and has room for seven bits, so 0x4300 | low seven bits is 128 + those, and what is to be
-// taken off is 128, or 256 (0x4380) where the code's sign bit says that it stands for 128 less.
-__device__ __forceinline__ uint32_t codes_to_bf16(uint32_t x) {
-  const uint32_t a = (x & 0x007f007fu) | 0x43004300u, b = (x & 0x00800080u) | 0x43004300u;
-  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
+__device__ __forceinline__ uint32_t f16_pair(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
+__device__ __forceinline__ uint32_t as_bits(__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); }
+// Four codes (offset by 128: the sign bit turned over) as two pairs of half-precision numbers: 0x6400 is 1024 and has room for ten bits.
+__device__ __forceinline__ void codes_to_f16(uint32_t w, __half2& a, __half2& b) {
+  const __half2 off = as_half2(0x64806480u);                     // 1024 + 128
+  const uint32_t x = w ^ 0x80808080u;
+  a = __hsub2(as_half2(__byte_perm(x, 0x64646464u, 0x4140)), off);
+  b = __hsub2(as_half2(__byte_perm(x, 0x64646464u, 0x4342)), off);
+}
+// The exponent of the largest of a page's 64 scales that is finite, a lane two of them; `none` where all are zero.
+__device__ __forceinline__ int top_exponent(float u, float v, int none) {
+  const uint32_t x = __float_as_uint(u) & 0x7fffffffu, y = __float_as_uint(v) & 0x7fffffffu;
+  const uint32_t top = __reduce_max_sync(0xffffffffu, max(x < 0x7f800000u ? x : 0u, y < 0x7f800000u ? y : 0u)) >> 23;
+  return top == 0 ? none : (int)top - 127;                       // (scales below the smallest normal number count as zeros here)
+}
+__device__ __forceinline__ float power_of_2(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
+__host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool b_mn_major) {
+  return (1u << 4) | (b_mn_major ? (1u << 16) : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 __device__ __forceinline__ uint64_t v_descriptor(uint32_t smem_addr, uint32_t block) {      // keys are the product's K, 128 contiguous bytes are 64 of its columns
   return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | (uint64_t)(block >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
@@ -121,16 +140,17 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
   uint8_t* q_tiles = smem;
   uint8_t* kv_tiles = smem + L::OFF_KV;
   uint8_t* raw_tiles = smem + L::OFF_RAW;
-  float* scales = reinterpret_cast<float*>(smem + L::OFF_SC);   // [SCALE_SETS][keys' (times scale and log2 e), logarithms of values', values' inverses][128]
+  uint8_t* sets = smem + L::OFF_SC;                              // [SCALE_SETS]: of two pages {2^(b - 8), c, 2^-c, whether a value's scale is not finite}, then a mark a key
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
-  uint64_t* kv_full = q_full + 1;                                // [RING] keys or values of a step are bfloat16
+  uint64_t* kv_full = q_full + 1;                                // [RING] keys or values of a step are half precision
   uint64_t* kv_empty = kv_full + RING;                           // [RING] both slots' products have read them
   uint64_t* raw_full = kv_empty + RING;                          // [RAW] a page's codes and scales have come
   uint64_t* raw_empty = raw_full + RAW;                          // [RAW] they have been turned
   uint64_t* s_full = raw_empty + RAW;                            // [slot] S is in tensor memory
   uint64_t* p_full = s_full + 2;                                 // [slot] P is (and S has been read)
   uint64_t* t_full = p_full + 2;                                 // [slot] P V has been added
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(t_full + 2);
+  uint64_t* q_ready = t_full + 2;                                // [slot] its queries are half precision
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_ready + 2);
   __shared__ int failed;
 
   pdl_launch_dependents();
@@ -159,7 +179,7 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
     mbar_init(q_full, 1);
     for (int i = 0; i < RING; ++i) { mbar_init(&kv_full[i], 128); mbar_init(&kv_empty[i], 2); }
     for (int i = 0; i < RAW; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 4); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); mbar_init(&t_full[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); mbar_init(&t_full[i], 1); mbar_init(&q_ready[i], 128); }
     failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_shared();
@@ -189,12 +209,10 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
             const int64_t cell = ((int64_t)pages[page_of(u)] * a.kv_heads + kvh) * PAGE;
             if (!mbar_wait(&raw_empty[r], phase)) { ok = false; break; }
             uint8_t* dst = raw_tiles + r * L::RAW_BYTES;
-            mbar_expect_tx(&raw_full[r], L::CODES + (x < 2 ? 2 * PAGE * 4 : 0));
+            mbar_expect_tx(&raw_full[r], L::CODES + (x < 2 ? 2 : 1) * PAGE * 4);
             if (!(a.skip_copy && u == 0 && x == 0)) bulk_copy(dst, (x < 2 ? a.k : a.v) + cell * HD, L::CODES, &raw_full[r]);
-            if (x < 2) {                                         // both scales with the keys: scores want both
-              bulk_copy(dst + L::CODES, a.ks + cell, PAGE * 4, &raw_full[r]);
-              bulk_copy(dst + L::CODES + PAGE * 4, a.vs + cell, PAGE * 4, &raw_full[r]);
-            }
+            bulk_copy(dst + L::CODES, a.vs + cell, PAGE * 4, &raw_full[r]);      // (values' scales with the keys too: scores want the pages' exponents)
+            if (x < 2) bulk_copy(dst + L::CODES + PAGE * 4, a.ks + cell, PAGE * 4, &raw_full[r]);
             if (++r == RAW) r = 0, phase ^= 1;
           }
         }
@@ -203,7 +221,7 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
       // ---- the products of a slot.  S of the next step goes over P, so it waits until P V has read it: meanwhile the tensor core works on the other slot
       const int t = warp - 1;
       const int mine = t == 0 ? (units0 + 1) / 2 : (units1 + 1) / 2;
-      constexpr uint32_t idesc_s = umma_instr_desc(ROWS, KEYS), idesc_t = umma_instr_desc(ROWS, HD, false, true);
+      constexpr uint32_t idesc_s = idesc_f16(ROWS, KEYS, false), idesc_t = idesc_f16(ROWS, HD, true);
       const bool one = elect_one();
       const uint64_t q_desc = sw128_desc(smem_u32(q_tiles + t * L::Q_BYTES)), k_desc = sw128_desc(smem_u32(kv_tiles));
       const uint64_t v_desc = v_descriptor(smem_u32(kv_tiles), L::BLOCK);
@@ -211,7 +229,7 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
       int r = 0;
       uint32_t phase = 0;
       auto next = [&] { if (++r == RING) r = 0, phase ^= 1; };
-      if (mine > 0) ok = mbar_wait(q_full, 0);
+      if (mine > 0) ok = mbar_wait(&q_ready[t], 0);
       for (int i = 0; i < steps && ok; ++i) {
         if (i < mine) {
           if (i > 0 && !mbar_wait(&t_full[t], (i - 1) & 1)) { ok = false; break; }
@@ -248,21 +266,42 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
       }
     }
   } else if (warp < 8) {
-    // ---- codes to bfloat16
+    // ---- codes to half precision
     regs_fewer<REGS_TURN>();
     const int tid = threadIdx.x - 128;
-    int raw = 0, r = 0;
+    int raw = 0, r = 0, exponent = -64, exponents[2] = {-64, -64};        // (a page of zeros takes the exponent of the values before it)
     uint32_t raw_phase = 0, phase = 1;
     for (int i = 0; i < steps && ok; ++i) {
-      for (int x = 0; x < 2 && ok; ++x) {                        // keys, values
-        if (!mbar_wait(&kv_empty[r], phase)) { ok = false; break; }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {                              // keys, values
+        if (!ok || !mbar_wait(&kv_empty[r], phase)) { ok = false; break; }
         uint8_t* dst = kv_tiles + r * L::KV_BYTES;
-        float* sc = scales + (i % SCALE_SETS) * 3 * KEYS;
+        uint8_t* set = sets + (i % SCALE_SETS) * L::SET;
+#pragma unroll
         for (int h = 0; h < 2; ++h) {                            // two pages
           const int u = 2 * i + h;
           if (u < units) {
-            if (!mbar_wait(&raw_full[raw], raw_phase)) { ok = false; break; }
+            if (!ok || !mbar_wait(&raw_full[raw], raw_phase)) { ok = false; break; }
             const uint8_t* src = raw_tiles + raw * L::RAW_BYTES;
+            const float* vs = reinterpret_cast<const float*>(src + L::CODES);
+            const float* ks = vs + PAGE;
+            const int there = min(PAGE, kv_len - page_of(u) * PAGE);      // beyond the sequence's end a scale may be anything
+            float shift;
+            if (x == 0) {
+              const float v0 = lane < there ? vs[lane] : 0.f, v1 = lane + 32 < there ? vs[lane + 32] : 0.f;
+              exponents[h] = exponent = top_exponent(v0, v1, exponent);
+              const int e = top_exponent(lane < there ? ks[lane] * a.scale_log2 : 0.f, lane + 32 < there ? ks[lane + 32] * a.scale_log2 : 0.f, 0);
+              shift = power_of_2(-e);
+              const bool b0 = !(fabsf(v0) < INFINITY), b1 = !(fabsf(v1) < INFINITY), bad = __any_sync(0xffffffffu, b0 || b1);
+              if (warp == 4) {
+                float* mark = reinterpret_cast<float*>(set + 32) + h * PAGE;
+                mark[lane] = b0 ? __uint_as_float(0x7fffffffu) : 0.f;
+                mark[lane + 32] = b1 ? __uint_as_float(0x7fffffffu) : 0.f;
+                if (lane == 0) reinterpret_cast<float4*>(set)[h] = make_float4(power_of_2(e) / SHIFT, (float)exponent, power_of_2(-exponent), bad ? 1.f : 0.f);
+              }
+            } else {
+              shift = power_of_2(-exponents[h]);
+            }
             constexpr int PER_ROW = HD / 16, PIECES = PAGE * PER_ROW;
             // a thread takes 16 codes; threads are dealt out so that eight neighbours read 128 bytes in a row and write pieces that lie in eight different banks' columns
 #pragma unroll
@@ -280,28 +319,22 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
                 }
                 const int4 w = *reinterpret_cast<const int4*>(src + row * HD + c * 16);
                 const uint32_t word[4] = {(uint32_t)w.x, (uint32_t)w.y, (uint32_t)w.z, (uint32_t)w.w};
+                float f = row < there ? (x == 0 ? ks[row] * a.scale_log2 : vs[row]) * shift * SHIFT : 0.f;
+                if (x == 1 && !(fabsf(f) < INFINITY)) f = 0.f;   // (its weight says so)
+                const __half2 hi = __float2half2_rn(f);
+                const __half2 lo = __float2half2_rn(f - __low2float(hi));
                 uint32_t e[8];
 #pragma unroll
                 for (int y = 0; y < 4; ++y) {
-                  e[2 * y] = codes_to_bf16(__byte_perm(word[y], 0, 0x4140));
-                  e[2 * y + 1] = codes_to_bf16(__byte_perm(word[y], 0, 0x4342));
+                  __half2 m, n;
+                  codes_to_f16(word[y], m, n);
+                  e[2 * y] = as_bits(x == 0 ? __hfma2(m, hi, __hmul2(m, lo)) : __hmul2(m, hi));
+                  e[2 * y + 1] = as_bits(x == 0 ? __hfma2(n, hi, __hmul2(n, lo)) : __hmul2(n, hi));
                 }
                 const int key = h * PAGE + row, piece = (c & 3) * 2;
                 uint8_t* d = dst + (c >> 2) * L::BLOCK + key * 128;
                 *reinterpret_cast<uint4*>(d + ((piece ^ (key & 7)) << 4)) = make_uint4(e[0], e[1], e[2], e[3]);
                 *reinterpret_cast<uint4*>(d + (((piece + 1) ^ (key & 7)) << 4)) = make_uint4(e[4], e[5], e[6], e[7]);
-              }
-            }
-            if (x == 0) {                                        // (beyond the sequence's end a scale may be anything)
-              const int key = tid & (PAGE - 1);
-              const bool there = page_of(u) * PAGE + key < kv_len;
-              const float v = there ? reinterpret_cast<const float*>(src + L::CODES)[tid] : 1.f;
-              if (tid < PAGE) {
-                sc[h * PAGE + key] = v * a.scale_log2;
-              } else {
-                const float w = v < LEAST ? LEAST : v;           // (not a number stays what it is)
-                sc[KEYS + h * PAGE + key] = log2f(w);
-                sc[2 * KEYS + h * PAGE + key] = 1.f / w;
               }
             }
             __syncwarp();
@@ -310,7 +343,8 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
           } else {                                               // no second page: keys of zeros
             for (int p = tid; p < L::BLOCKS * PAGE * 8; p += 128)
               *reinterpret_cast<uint4*>(dst + (p / (PAGE * 8)) * L::BLOCK + PAGE * 128 + (p % (PAGE * 8)) * 16) = make_uint4(0, 0, 0, 0);
-            if (x == 0 && tid < PAGE) sc[PAGE + tid] = sc[KEYS + PAGE + tid] = sc[2 * KEYS + PAGE + tid] = 1.f;
+            if (x == 0 && tid < PAGE) reinterpret_cast<float*>(set + 32)[PAGE + tid] = 0.f;
+            if (x == 0 && tid == 0) reinterpret_cast<float4*>(set)[1] = make_float4(1.f, (float)exponent, power_of_2(-exponent), 0.f);
           }
         }
         if (!ok) break;
@@ -331,44 +365,73 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
     auto whole = [&](int page) {
       return page * PAGE + PAGE - 1 <= first_pos && (a.window == 0 || page * PAGE > last_pos - a.window || page * PAGE + PAGE <= a.keep_first);
     };
-    float ref = -INFINITY;                       // what the weights are relative to: the row's maximum, or up to RISE less
-    uint64_t sum[2] = {0, 0};
-    for (int i = 0; i < mine; ++i) {
+    float row_mul = 1.f;
+    if (mine > 0) {                                              // the row's queries to half precision, in place
+      ok = mbar_wait(q_full, 0);
+      uint8_t* q = q_tiles + t * L::Q_BYTES + row * 128;
+      uint4 x[HD / 8];
+      uint32_t top = 0;
+#pragma unroll
+      for (int c = 0; c < HD / 8; ++c) {
+        x[c] = *reinterpret_cast<const uint4*>(q + (c >> 3) * L::BLOCK + (((c & 7) ^ (row & 7)) << 4));
+        top = __vmaxu2(top, __vmaxu2(__vmaxu2(x[c].x & 0x7fff7fffu, x[c].y & 0x7fff7fffu), __vmaxu2(x[c].z & 0x7fff7fffu, x[c].w & 0x7fff7fffu)));
+      }
+      const uint32_t e = max(top & 0xffffu, top >> 16) >> 7;     // its largest exponent
+      const uint32_t used = e == 255 ? 127u : min(max(e, 1u), 253u);      // (a row that is not finite stays so)
+      const float f = __uint_as_float((254u - used) << 23);
+      row_mul = __uint_as_float(used << 23);
+#pragma unroll
+      for (int c = 0; c < HD / 8; ++c) {
+        uint32_t w[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+#pragma unroll
+        for (int y = 0; y < 4; ++y) w[y] = f16_pair(__uint_as_float(w[y] << 16) * f, __uint_as_float(w[y] & 0xffff0000u) * f);
+        *reinterpret_cast<uint4*>(q + (c >> 3) * L::BLOCK + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      fence_async_shared();
+      mbar_arrive_one(&q_ready[t]);
+    }
+    float ref = -INFINITY, sum = 0.f;            // what the weights are relative to: the row's largest t + c, or up to RISE less
+    for (int i = 0; i < mine && ok; ++i) {
       const int page0 = page_of(2 * i), page1 = 2 * i + 1 < units ? page_of(2 * i + 1) : 1 << 24;      // (no second page: keys that nobody sees)
-      const bool masked = !(whole(page0) && 2 * i + 1 < units && whole(page1));
-      const float* ks = scales + (i % SCALE_SETS) * 3 * KEYS;
-      const float* vl = ks + KEYS;
-      const float* vi = vl + KEYS;
+      const uint8_t* set = sets + (i % SCALE_SETS) * L::SET;
       if (!mbar_wait(&s_full[t], i & 1)) { ok = false; break; }
       tc_fence_after();
-      uint32_t x[KEYS];                          // the row's scores, in place
-      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      const float4 about0 = reinterpret_cast<const float4*>(set)[0], about1 = reinterpret_cast<const float4*>(set)[1];
+      const float mul0 = fmaxf(about0.x * row_mul, 0x1p-126f), mul1 = fmaxf(about1.x * row_mul, 0x1p-126f);
+      const bool marked = about0.w + about1.w > 0.f;
+      const bool look = marked || !(whole(page0) && 2 * i + 1 < units && whole(page1));
+      // The row's scores of a page.  They are read twice, for the maximum and for the weights: 128 of them do not fit a thread's registers beside what else it needs.
+      auto scores = [&](int h, uint32_t (&x)[PAGE]) {
+        tmem_ld32(tm_s + h * PAGE, x);
+        tmem_ld32(tm_s + h * PAGE + 32, x + 32);
+        tmem_ld_wait();
+        if (look) {
+          const float* mark = reinterpret_cast<const float*>(set + 32) + h * PAGE;
+          const int key0 = (h ? page1 : page0) * PAGE;
 #pragma unroll
-      for (int c0 = 0; c0 < KEYS; c0 += 32) tmem_ld32(tm_s + c0, x + c0);
-      tmem_ld_wait();
-#pragma unroll
-      for (int c = 0; c < KEYS; c += 4) {
-        const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(ks + c), g = *reinterpret_cast<const ulonglong2*>(vl + c);
-        scale_pair(x + c, f.x, g.x);
-        scale_pair(x + c + 2, f.y, g.y);
-      }
-      if (masked) {
-#pragma unroll
-        for (int c = 0; c < KEYS; ++c) {
-          const int key = (c < PAGE ? page0 * PAGE : page1 * PAGE - PAGE) + c;
-          if (!(key <= pos && (a.window == 0 || pos - key < a.window || key < a.keep_first))) x[c] = 0xff800000u;
+          for (int c = 0; c < PAGE; ++c) {
+            const int key = key0 + c;
+            const bool sees = key <= pos && (a.window == 0 || pos - key < a.window || key < a.keep_first);
+            x[c] = sees ? __float_as_uint(__uint_as_float(x[c]) + mark[c]) : 0xff800000u;
+          }
         }
-      }
+      };
+      float top[2];
 #pragma unroll
-      for (int c = 0; c < KEYS; c += 2) top[(c >> 1) & 3] = fmaxf(top[(c >> 1) & 3], fmaxf(__uint_as_float(x[c]), __uint_as_float(x[c + 1])));
-      const float peak = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      for (int h = 0; h < 2; ++h) {
+        uint32_t x[PAGE];
+        scores(h, x);
+        float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < PAGE; c += 2) m[(c >> 1) & 3] = fmaxf(fmaxf(m[(c >> 1) & 3], __uint_as_float(x[c])), __uint_as_float(x[c + 1]));
+        top[h] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+      }
+      const float peak = fmaxf(fmaf(top[0], mul0, about0.y), fmaf(top[1], mul1, about1.y));
       if (i == 0) {
         ref = peak;
       } else if (__any_sync(0xffffffffu, peak > ref + RISE)) {   // (S of this step was begun after P V of the last had ended: the output is at rest)
         const float to = fmaxf(ref, peak), keep = ref == -INFINITY ? 0.f : exp2_fast(ref - to);
-        const uint64_t keep2 = pair(keep, keep);
-        sum[0] = fma2(sum[0], keep2, 0);
-        sum[1] = fma2(sum[1], keep2, 0);
+        sum *= keep;
         ref = to;
 #pragma unroll
         for (int c0 = 0; c0 < HD; c0 += 16) {
@@ -381,32 +444,30 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
           tmem_st8(tm_o + c0 + 8, w[1]);
         }
       }
-      const float base = ref == -INFINITY ? 0.f : -ref;          // a row that has seen nothing yet
-      const uint64_t base2 = pair(base, base);
+      const float base = HEAD - (ref == -INFINITY ? 0.f : ref);  // (a row that has seen nothing yet)
 #pragma unroll
-      for (int c0 = 0; c0 < KEYS; c0 += 16) {
-        uint32_t w[8];
+      for (int h = 0; h < 2; ++h) {
+        const uint64_t mul = h ? pair(mul1, mul1) : pair(mul0, mul0), add = h ? pair(about1.y + base, about1.y + base) : pair(about0.y + base, about0.y + base);
+        uint64_t part[2] = {0, 0};
+        uint32_t x[PAGE];
+        scores(h, x);
 #pragma unroll
-        for (int c = 0; c < 16; c += 4) {
-          const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(vi + c0 + c);
+        for (int c0 = 0; c0 < PAGE; c0 += 16) {
+          uint32_t w[8];
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float u = __uint_as_float(x[c0 + c + 2 * e]), v = __uint_as_float(x[c0 + c + 2 * e + 1]);
+          for (int c = 0; c < 8; ++c) {
             float p, q;
-            halves(add2(pair(u, v), base2), p, q);
+            halves(fma2(pair(__uint_as_float(x[c0 + 2 * c]), __uint_as_float(x[c0 + 2 * c + 1])), mul, add), p, q);
             p = exp2_fast(p);
             q = exp2_fast(q);
-            uint64_t g = e ? f.y : f.x;
-            if (masked) {                                        // (a scale that is not finite is for those alone who see it)
-              float y, z;
-              halves(g, y, z);
-              g = pair(u == -INFINITY ? 0.f : y, v == -INFINITY ? 0.f : z);
-            }
-            sum[e] = fma2(pair(p, q), g, sum[e]);
-            w[c / 2 + e] = bf16_pair(p, q);
+            part[c & 1] = add2(part[c & 1], pair(p, q));
+            w[c] = f16_pair(p, q);
           }
+          tmem_st8(tm_s + (h * PAGE + c0) / 2, w);      // (over scores that have been read: the second page's begin at column 64)
         }
-        tmem_st8(tm_s + c0 / 2, w);
+        float u, v;
+        halves(add2(part[0], part[1]), u, v);
+        sum = fmaf(u + v, h ? about1.z : about0.z, sum);
       }
       tmem_st_wait();
       tc_fence_before();
@@ -415,10 +476,7 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
     if (ok && mine > 0) {
       ok = mbar_wait(&t_full[t], (mine - 1) & 1);
       tc_fence_after();
-      float u, v, u1, v1;
-      halves(sum[0], u, v);
-      halves(sum[1], u1, v1);
-      const float inv = 1.f / ((u + v) + (u1 + v1));
+      const float inv = 1.f / (sum * SHIFT);
       const int token = row / group, head = row - token * group;
       const bool there = ok && token < n_tok && !failed;
       __nv_bfloat16* dst = a.out + (int64_t)(row0 + tok0 + t * tok + token) * a.ld_out + (int64_t)(kvh * group + head) * HD;
