@@ -13,9 +13,11 @@
 // Scores, maxima, sums and outputs are 32-bit.
 //
 // A block has two SLOTS of 128 rows: rows are (token, head) pairs of one key/value head's group, so that the heads that share keys share the work of bringing them.
-// Keys come in steps of two pages (128).  Roles, by warp:
+// Keys come a page (64) at a time.  Roles, by warp:
 //   0       brings the queries by TMA and the pages' codes and scales, as they lie, by bulk copies into a ring
-//   1, 2    issue the products of a slot each:  S = Q K^T (128 x 128), then T += P V with P in tensor memory, over S's own columns
+//   1, 2    issue the products of a slot each: S = Q K^T of the next page (128 x 64, two places in turn) before T += P V of this one (P in tensor memory, over its
+//           S's own columns), so that a row's thread finds the next scores there when it is done with these.  (Steps of 128 keys with one place for S read Q
+//           half as often, but every step then waits for two products there and back: 7800 cycles for 128 keys of 256 rows.)
 //   4-7     turn codes to half precision in the layout the products read (128-byte swizzle), once for both slots' 256 rows: a code's byte under 0x64 is 1024 + code + 128
 //   8-11, 12-15  a thread a row: scores to weights.  The running output stays in tensor memory; it is scaled down only when a row's maximum has risen by
 //           more than 2^8 since the last time, which after the first steps is hardly ever
@@ -33,10 +35,9 @@ KVAD_DEFINE_LAST_ERROR()
 
 namespace {
 
-constexpr int KEYS = 128;                       // of a step: two pages
 constexpr int THREADS = 512;
-constexpr int REGS_FEW = 72, REGS_TURN = 104, REGS_MANY = 168;      // of 128 a thread at launch: 72 + 104 + 2 * 168 = 4 * 128
-constexpr int SCALE_SETS = 4;
+constexpr int REGS_FEW = 80, REGS_TURN = 96, REGS_MANY = 168;       // of 128 a thread at launch: 80 + 96 + 2 * 168 = 4 * 128
+constexpr int SETS = 8;
 constexpr float RISE = 8.f, HEAD = 6.f;      // weights are at most 2^(RISE + HEAD)
 constexpr float SHIFT = 256.f;                  // largest scaled code: below 127 * 2 * 2^8, under half precision's 65504
 
@@ -59,16 +60,16 @@ struct Args {
 
 template <int HD> struct Layout {
   static constexpr int BLOCKS = (HD + 63) / 64;                  // of 64 entries: 128 bytes
-  static constexpr int RING = HD > 64 ? 3 : 6, RAW = 6;         // keys or values of a step in half precision; of a page as they came
-  static constexpr uint32_t BLOCK = 128 * 128;                   // 128 rows (or keys) of a block of entries
-  static constexpr uint32_t Q_BYTES = BLOCKS * BLOCK, KV_BYTES = BLOCKS * BLOCK;
+  static constexpr int RING = HD > 64 ? 6 : 8, RAW = 6;         // pages of keys or values in half precision, and as they came
+  static constexpr uint32_t Q_BYTES = BLOCKS * Q_BLOCK, KV_BYTES = BLOCKS * PAGE_BLOCK;
   static constexpr uint32_t CODES = PAGE * HD, RAW_BYTES = CODES + 2 * PAGE * 4;
-  static constexpr uint32_t SET = 32 + KEYS * 4;                 // of a step: what softmax threads need of its two pages, and marks of its keys
+  static constexpr uint32_t SET = 16 + PAGE * 4;                 // what softmax threads need of a page, and marks of its keys
   static constexpr uint32_t OFF_KV = 2 * Q_BYTES, OFF_RAW = OFF_KV + RING * KV_BYTES, OFF_SC = OFF_RAW + RAW * RAW_BYTES;
-  static constexpr uint32_t OFF_BAR = OFF_SC + SCALE_SETS * SET;
-  static constexpr int BARS = 1 + 2 * RING + 2 * RAW + 2 * 4;
+  static constexpr uint32_t OFF_BAR = OFF_SC + SETS * SET;
+  static constexpr int BARS = 1 + 2 * RING + 2 * RAW + 2 * 6;
   static constexpr size_t SMEM = OFF_BAR + BARS * 8 + 16 + 1024;
-  static constexpr uint32_t TM_O = 2 * KEYS;                     // S (and P) of slot t at t * 128, its output at TM_O + t * 128
+  static constexpr uint32_t TM_O = 256;                          // S (and P) of slot t at t * 128 + 64 in turn, its output at TM_O + t * 128
+  static_assert(SETS >= RING / 2 + 2, "a page's set is read until the products of the page before are done");
   static_assert(SMEM <= 227 * 1024, "an SM's shared memory");
 };
 
@@ -126,10 +127,6 @@ __device__ __forceinline__ float power_of_2(int e) { return __uint_as_float((uin
 __host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool b_mn_major) {
   return (1u << 4) | (b_mn_major ? (1u << 16) : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
-__device__ __forceinline__ uint64_t v_descriptor(uint32_t smem_addr, uint32_t block) {      // keys are the product's K, 128 contiguous bytes are 64 of its columns
-  return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | (uint64_t)(block >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
-
 template <int HD>
 __global__ void __launch_bounds__(THREADS, 1)
 attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ Args a) {
@@ -140,15 +137,15 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
   uint8_t* q_tiles = smem;
   uint8_t* kv_tiles = smem + L::OFF_KV;
   uint8_t* raw_tiles = smem + L::OFF_RAW;
-  uint8_t* sets = smem + L::OFF_SC;                              // [SCALE_SETS]: of two pages {2^(b - 8), c, 2^-c, whether a value's scale is not finite}, then a mark a key
+  uint8_t* sets = smem + L::OFF_SC;                              // [SETS]: of a page {2^(b - 8), c, 2^-c, whether a value's scale is not finite}, then a mark a key
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
-  uint64_t* kv_full = q_full + 1;                                // [RING] keys or values of a step are half precision
+  uint64_t* kv_full = q_full + 1;                                // [RING] a page's keys or values are half precision
   uint64_t* kv_empty = kv_full + RING;                           // [RING] both slots' products have read them
   uint64_t* raw_full = kv_empty + RING;                          // [RAW] a page's codes and scales have come
   uint64_t* raw_empty = raw_full + RAW;                          // [RAW] they have been turned
-  uint64_t* s_full = raw_empty + RAW;                            // [slot] S is in tensor memory
-  uint64_t* p_full = s_full + 2;                                 // [slot] P is (and S has been read)
-  uint64_t* t_full = p_full + 2;                                 // [slot] P V has been added
+  uint64_t* s_full = raw_empty + RAW;                            // [slot][2] S is in tensor memory
+  uint64_t* p_full = s_full + 4;                                 // [slot][2] P is (and S has been read)
+  uint64_t* t_full = p_full + 4;                                 // [slot] P V has been added
   uint64_t* q_ready = t_full + 2;                                // [slot] its queries are half precision
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_ready + 2);
   __shared__ int failed;
@@ -171,7 +168,7 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
   const int kept = min((a.keep_first + PAGE - 1) / PAGE, first_page);
   const int units0 = kept + (pos0 + n_tok0 - 1) / PAGE - first_page + 1;
   const int units1 = n_tok1 > 0 ? kept + (pos0 + tok + n_tok1 - 1) / PAGE - first_page + 1 : 0;
-  const int units = max(units0, units1), steps = (units + 1) / 2;
+  const int units = max(units0, units1);
   auto page_of = [&](int u) { return u < kept ? u : first_page + u - kept; };
 
   if (threadIdx.x == 0) {
@@ -179,7 +176,8 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
     mbar_init(q_full, 1);
     for (int i = 0; i < RING; ++i) { mbar_init(&kv_full[i], 128); mbar_init(&kv_empty[i], 2); }
     for (int i = 0; i < RAW; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 4); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); mbar_init(&t_full[i], 1); mbar_init(&q_ready[i], 128); }
+    for (int i = 0; i < 4; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&t_full[i], 1); mbar_init(&q_ready[i], 128); }
     failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_shared();
@@ -199,69 +197,72 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
         mbar_expect_tx(q_full, (n_tok1 > 0 ? 2u : 1u) * L::BLOCKS * box);
         for (int t = 0; t < (n_tok1 > 0 ? 2 : 1); ++t)
           for (int b = 0; b < L::BLOCKS; ++b)
-            tma_load_3d(q_tiles + t * L::Q_BYTES + b * L::BLOCK, &map_q, q_full, b * 64, kvh * group, row0 + tok0 + t * tok);
+            tma_load_3d(q_tiles + t * L::Q_BYTES + b * Q_BLOCK, &map_q, q_full, b * 64, kvh * group, row0 + tok0 + t * tok);
         int r = 0;
         uint32_t phase = 1;                                      // (the first round finds the ring empty)
-        for (int u0 = 0; u0 < units && ok; u0 += 2) {
-          for (int x = 0; x < 4; ++x) {                          // keys of two pages, then their values
-            const int u = u0 + (x & 1);
-            if (u >= units) continue;
-            const int64_t cell = ((int64_t)pages[page_of(u)] * a.kv_heads + kvh) * PAGE;
-            if (!mbar_wait(&raw_empty[r], phase)) { ok = false; break; }
-            uint8_t* dst = raw_tiles + r * L::RAW_BYTES;
-            mbar_expect_tx(&raw_full[r], L::CODES + (x < 2 ? 2 : 1) * PAGE * 4);
-            if (!(a.skip_copy && u == 0 && x == 0)) bulk_copy(dst, (x < 2 ? a.k : a.v) + cell * HD, L::CODES, &raw_full[r]);
-            bulk_copy(dst + L::CODES, a.vs + cell, PAGE * 4, &raw_full[r]);      // (values' scales with the keys too: scores want the pages' exponents)
-            if (x < 2) bulk_copy(dst + L::CODES + PAGE * 4, a.ks + cell, PAGE * 4, &raw_full[r]);
-            if (++r == RAW) r = 0, phase ^= 1;
-          }
+        // keys of page 0, then keys of the next page and values of this one in turn: the order of use
+        for (int n = 0; n < 2 * units && ok; ++n) {
+          const bool values = n == 2 * units - 1 || (n > 0 && (n & 1) == 0);
+          const int u = n == 2 * units - 1 ? units - 1 : values ? n / 2 - 1 : (n + 1) / 2;
+          const int64_t cell = ((int64_t)pages[page_of(u)] * a.kv_heads + kvh) * PAGE;
+          if (!mbar_wait(&raw_empty[r], phase)) { ok = false; break; }
+          uint8_t* dst = raw_tiles + r * L::RAW_BYTES;
+          mbar_expect_tx(&raw_full[r], L::CODES + (values ? 1 : 2) * PAGE * 4);
+          if (!(a.skip_copy && n == 0)) bulk_copy(dst, (values ? a.v : a.k) + cell * HD, L::CODES, &raw_full[r]);
+          bulk_copy(dst + L::CODES, a.vs + cell, PAGE * 4, &raw_full[r]);        // (values' scales with the keys too: scores want the pages' exponents)
+          if (!values) bulk_copy(dst + L::CODES + PAGE * 4, a.ks + cell, PAGE * 4, &raw_full[r]);
+          if (++r == RAW) r = 0, phase ^= 1;
         }
       }
     } else if (warp < 3) {
-      // ---- the products of a slot.  S of the next step goes over P, so it waits until P V has read it: meanwhile the tensor core works on the other slot
-      const int t = warp - 1;
-      const int mine = t == 0 ? (units0 + 1) / 2 : (units1 + 1) / 2;
-      constexpr uint32_t idesc_s = idesc_f16(ROWS, KEYS, false), idesc_t = idesc_f16(ROWS, HD, true);
+      // ---- the products of a slot
+      const int t = warp - 1, mine = t == 0 ? units0 : units1;
+      constexpr uint32_t idesc_s = idesc_f16(ROWS, PAGE, false), idesc_t = idesc_f16(ROWS, HD, true);
       const bool one = elect_one();
       const uint64_t q_desc = sw128_desc(smem_u32(q_tiles + t * L::Q_BYTES)), k_desc = sw128_desc(smem_u32(kv_tiles));
-      const uint64_t v_desc = v_descriptor(smem_u32(kv_tiles), L::BLOCK);
-      const uint32_t tm_s = tmem + t * KEYS, tm_o = tmem + L::TM_O + t * 128;
+      const uint64_t v_desc = sw128_mn_desc(smem_u32(kv_tiles));
+      const uint32_t tm_s = tmem + t * 128, tm_o = tmem + L::TM_O + t * 128;
       int r = 0;
       uint32_t phase = 0;
       auto next = [&] { if (++r == RING) r = 0, phase ^= 1; };
       if (mine > 0) ok = mbar_wait(&q_ready[t], 0);
-      for (int i = 0; i < steps && ok; ++i) {
-        if (i < mine) {
-          if (i > 0 && !mbar_wait(&t_full[t], (i - 1) & 1)) { ok = false; break; }
+      // keys of page i + 1, then values of page i: from page -1 on, which has no values, to the last, which has no next
+      for (int i = -1; i < units && ok; ++i) {
+        if (i + 1 < units) {
+          if (i + 1 < mine && i > 0 && !mbar_wait(&t_full[t], (i - 1) & 1)) { ok = false; break; }      // P V of page i - 1 has read what S goes over
           if (!mbar_wait(&kv_full[r], phase)) { ok = false; break; }
-          tc_fence_after();
-          if (one) {
-            const uint64_t at = k_desc + (uint32_t)r * (L::KV_BYTES >> 4);
+          if (i + 1 < mine) {
+            tc_fence_after();
+            if (one) {
+              const uint64_t at = k_desc + (uint32_t)r * (L::KV_BYTES >> 4);
 #pragma unroll
-            for (int k = 0; k < HD / 16; ++k) {
-              const uint64_t off = (uint64_t)((k / 4) * (L::BLOCK >> 4) + (k % 4) * 2);
-              umma(tm_s, q_desc + off, at + off, idesc_s, k > 0 ? 1u : 0u);
+              for (int k = 0; k < HD / 16; ++k)
+                umma(tm_s + ((i + 1) & 1) * PAGE, q_desc + (uint64_t)((k / 4) * (Q_BLOCK >> 4) + (k % 4) * 2), at + (uint64_t)((k / 4) * (PAGE_BLOCK >> 4) + (k % 4) * 2),
+                     idesc_s, k > 0 ? 1u : 0u);
+              umma_commit(&s_full[t * 2 + ((i + 1) & 1)]);
+              umma_commit(&kv_empty[r]);
             }
-            umma_commit(&s_full[t]);
-            umma_commit(&kv_empty[r]);
+          } else if (lane == 0) {
+            mbar_arrive_one(&kv_empty[r]);                       // (the other slot walks on: what comes goes back unread)
           }
           next();
-          if (!(mbar_wait(&p_full[t], i & 1) && mbar_wait(&kv_full[r], phase))) { ok = false; break; }
-          tc_fence_after();
-          if (one) {
-            const uint64_t at = v_desc + (uint32_t)r * (L::KV_BYTES >> 4);
+        }
+        if (i >= 0) {
+          if (i < mine && !mbar_wait(&p_full[t * 2 + (i & 1)], (i >> 1) & 1)) { ok = false; break; }
+          if (!mbar_wait(&kv_full[r], phase)) { ok = false; break; }
+          if (i < mine) {
+            tc_fence_after();
+            if (one) {
+              const uint64_t at = v_desc + (uint32_t)r * (L::KV_BYTES >> 4);
 #pragma unroll
-            for (int k = 0; k < KEYS / 16; ++k) umma_ta(tm_o, tm_s + k * 8, at + (uint64_t)(k * (2048 >> 4)), idesc_t, (i > 0 || k > 0) ? 1u : 0u);
-            umma_commit(&t_full[t]);
-            umma_commit(&kv_empty[r]);
+              for (int k = 0; k < PAGE / 16; ++k) umma_ta(tm_o, tm_s + (i & 1) * PAGE + k * 8, at + (uint64_t)(k * (2048 >> 4)), idesc_t, (i > 0 || k > 0) ? 1u : 0u);
+              umma_commit(&t_full[t]);
+              umma_commit(&kv_empty[r]);
+            }
+          } else if (lane == 0) {
+            mbar_arrive_one(&kv_empty[r]);
           }
           next();
-        } else {                                                 // the other slot walks on: give back what comes unread
-          for (int x = 0; x < 2 && ok; ++x) {
-            ok = mbar_wait(&kv_full[r], phase);
-            if (ok && lane == 0) mbar_arrive_one(&kv_empty[r]);
-            next();
-          }
         }
       }
     }
@@ -269,102 +270,88 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
     // ---- codes to half precision
     regs_fewer<REGS_TURN>();
     const int tid = threadIdx.x - 128;
-    int raw = 0, r = 0, exponent = -64, exponents[2] = {-64, -64};        // (a page of zeros takes the exponent of the values before it)
+    int raw = 0, r = 0, exponent = -64, before = -64;            // of values of the latest page and the one before (a page of zeros takes the one before's)
     uint32_t raw_phase = 0, phase = 1;
-    for (int i = 0; i < steps && ok; ++i) {
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {                              // keys, values
-        if (!ok || !mbar_wait(&kv_empty[r], phase)) { ok = false; break; }
-        uint8_t* dst = kv_tiles + r * L::KV_BYTES;
-        uint8_t* set = sets + (i % SCALE_SETS) * L::SET;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {                            // two pages
-          const int u = 2 * i + h;
-          if (u < units) {
-            if (!ok || !mbar_wait(&raw_full[raw], raw_phase)) { ok = false; break; }
-            const uint8_t* src = raw_tiles + raw * L::RAW_BYTES;
-            const float* vs = reinterpret_cast<const float*>(src + L::CODES);
-            const float* ks = vs + PAGE;
-            const int there = min(PAGE, kv_len - page_of(u) * PAGE);      // beyond the sequence's end a scale may be anything
-            float shift;
-            if (x == 0) {
-              const float v0 = lane < there ? vs[lane] : 0.f, v1 = lane + 32 < there ? vs[lane + 32] : 0.f;
-              exponents[h] = exponent = top_exponent(v0, v1, exponent);
-              const int e = top_exponent(lane < there ? ks[lane] * a.scale_log2 : 0.f, lane + 32 < there ? ks[lane + 32] * a.scale_log2 : 0.f, 0);
-              shift = power_of_2(-e);
-              const bool b0 = !(fabsf(v0) < INFINITY), b1 = !(fabsf(v1) < INFINITY), bad = __any_sync(0xffffffffu, b0 || b1);
-              if (warp == 4) {
-                float* mark = reinterpret_cast<float*>(set + 32) + h * PAGE;
-                mark[lane] = b0 ? __uint_as_float(0x7fffffffu) : 0.f;
-                mark[lane + 32] = b1 ? __uint_as_float(0x7fffffffu) : 0.f;
-                if (lane == 0) reinterpret_cast<float4*>(set)[h] = make_float4(power_of_2(e) / SHIFT, (float)exponent, power_of_2(-exponent), bad ? 1.f : 0.f);
-              }
-            } else {
-              shift = power_of_2(-exponents[h]);
-            }
-            constexpr int PER_ROW = HD / 16, PIECES = PAGE * PER_ROW;
-            // a thread takes 16 codes; threads are dealt out so that eight neighbours read 128 bytes in a row and write pieces that lie in eight different banks' columns
-#pragma unroll
-            for (int p0 = 0; p0 < PIECES; p0 += 128) {
-              const int p = p0 + tid;
-              if (PIECES % 128 == 0 || p < PIECES) {
-                int row, c;
-                if (PER_ROW == 8) {
-                  const int q = (p >> 2) & 3;
-                  row = (p >> 4) * 2 + (q & 1);
-                  c = (p & 3) + ((q == 1 || q == 2) ? 4 : 0);
-                } else {
-                  row = p / PER_ROW;
-                  c = p - row * PER_ROW;
-                }
-                const int4 w = *reinterpret_cast<const int4*>(src + row * HD + c * 16);
-                const uint32_t word[4] = {(uint32_t)w.x, (uint32_t)w.y, (uint32_t)w.z, (uint32_t)w.w};
-                float f = row < there ? (x == 0 ? ks[row] * a.scale_log2 : vs[row]) * shift * SHIFT : 0.f;
-                if (x == 1 && !(fabsf(f) < INFINITY)) f = 0.f;   // (its weight says so)
-                const __half2 hi = __float2half2_rn(f);
-                const __half2 lo = __float2half2_rn(f - __low2float(hi));
-                uint32_t e[8];
-#pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                  __half2 m, n;
-                  codes_to_f16(word[y], m, n);
-                  e[2 * y] = as_bits(x == 0 ? __hfma2(m, hi, __hmul2(m, lo)) : __hmul2(m, hi));
-                  e[2 * y + 1] = as_bits(x == 0 ? __hfma2(n, hi, __hmul2(n, lo)) : __hmul2(n, hi));
-                }
-                const int key = h * PAGE + row, piece = (c & 3) * 2;
-                uint8_t* d = dst + (c >> 2) * L::BLOCK + key * 128;
-                *reinterpret_cast<uint4*>(d + ((piece ^ (key & 7)) << 4)) = make_uint4(e[0], e[1], e[2], e[3]);
-                *reinterpret_cast<uint4*>(d + (((piece + 1) ^ (key & 7)) << 4)) = make_uint4(e[4], e[5], e[6], e[7]);
-              }
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive_one(&raw_empty[raw]);
-            if (++raw == RAW) raw = 0, raw_phase ^= 1;
-          } else {                                               // no second page: keys of zeros
-            for (int p = tid; p < L::BLOCKS * PAGE * 8; p += 128)
-              *reinterpret_cast<uint4*>(dst + (p / (PAGE * 8)) * L::BLOCK + PAGE * 128 + (p % (PAGE * 8)) * 16) = make_uint4(0, 0, 0, 0);
-            if (x == 0 && tid < PAGE) reinterpret_cast<float*>(set + 32)[PAGE + tid] = 0.f;
-            if (x == 0 && tid == 0) reinterpret_cast<float4*>(set)[1] = make_float4(1.f, (float)exponent, power_of_2(-exponent), 0.f);
-          }
+    auto turn = [&](auto which, int u) {                         // keys or values of page u
+      constexpr bool VALUES = decltype(which)::value;
+      if (!mbar_wait(&kv_empty[r], phase) || !mbar_wait(&raw_full[raw], raw_phase)) { ok = false; return; }
+      uint8_t* dst = kv_tiles + r * L::KV_BYTES;
+      const uint8_t* src = raw_tiles + raw * L::RAW_BYTES;
+      const float* vs = reinterpret_cast<const float*>(src + L::CODES);
+      const float* ks = vs + PAGE;
+      const int there = min(PAGE, kv_len - page_of(u) * PAGE);   // beyond the sequence's end a scale may be anything
+      float shift;
+      if (!VALUES) {
+        const float v0 = lane < there ? vs[lane] : 0.f, v1 = lane + 32 < there ? vs[lane + 32] : 0.f;
+        before = exponent;
+        exponent = top_exponent(v0, v1, exponent);
+        const int e = top_exponent(lane < there ? ks[lane] * a.scale_log2 : 0.f, lane + 32 < there ? ks[lane + 32] * a.scale_log2 : 0.f, 0);
+        shift = power_of_2(-e);
+        const bool b0 = !(fabsf(v0) < INFINITY), b1 = !(fabsf(v1) < INFINITY), bad = __any_sync(0xffffffffu, b0 || b1);
+        if (warp == 4) {
+          uint8_t* set = sets + (u % SETS) * L::SET;
+          float* mark = reinterpret_cast<float*>(set + 16);
+          mark[lane] = b0 ? __uint_as_float(0x7fffffffu) : 0.f;
+          mark[lane + 32] = b1 ? __uint_as_float(0x7fffffffu) : 0.f;
+          if (lane == 0) *reinterpret_cast<float4*>(set) = make_float4(power_of_2(e) / SHIFT, (float)exponent, power_of_2(-exponent), bad ? 1.f : 0.f);
         }
-        if (!ok) break;
-        fence_async_shared();
-        mbar_arrive_one(&kv_full[r]);
-        if (++r == RING) r = 0, phase ^= 1;
+      } else {
+        shift = power_of_2(u == units - 1 ? -exponent : -before);
       }
+      constexpr int PER_ROW = HD / 16, PIECES = PAGE * PER_ROW;
+      // a thread takes 16 codes; threads are dealt out so that eight neighbours read 128 bytes in a row and write pieces that lie in eight different banks' columns
+#pragma unroll
+      for (int p0 = 0; p0 < PIECES; p0 += 128) {
+        const int p = p0 + tid;
+        if (PIECES % 128 == 0 || p < PIECES) {
+          int row, c;
+          if (PER_ROW == 8) {
+            const int q = (p >> 2) & 3;
+            row = (p >> 4) * 2 + (q & 1);
+            c = (p & 3) + ((q == 1 || q == 2) ? 4 : 0);
+          } else {
+            row = p / PER_ROW;
+            c = p - row * PER_ROW;
+          }
+          const int4 w = *reinterpret_cast<const int4*>(src + row * HD + c * 16);
+          const uint32_t word[4] = {(uint32_t)w.x, (uint32_t)w.y, (uint32_t)w.z, (uint32_t)w.w};
+          float f = row < there ? (VALUES ? vs[row] : ks[row] * a.scale_log2) * shift * SHIFT : 0.f;
+          if (VALUES && !(fabsf(f) < INFINITY)) f = 0.f;         // (its weight says so)
+          const __half2 hi = __float2half2_rn(f);
+          const __half2 lo = __float2half2_rn(f - __low2float(hi));
+          uint32_t e[8];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            __half2 m, n;
+            codes_to_f16(word[y], m, n);
+            e[2 * y] = as_bits(VALUES ? __hmul2(m, hi) : __hfma2(m, hi, __hmul2(m, lo)));
+            e[2 * y + 1] = as_bits(VALUES ? __hmul2(n, hi) : __hfma2(n, hi, __hmul2(n, lo)));
+          }
+          const int piece = (c & 3) * 2;
+          uint8_t* d = dst + (c >> 2) * PAGE_BLOCK + row * 128;
+          *reinterpret_cast<uint4*>(d + ((piece ^ (row & 7)) << 4)) = make_uint4(e[0], e[1], e[2], e[3]);
+          *reinterpret_cast<uint4*>(d + (((piece + 1) ^ (row & 7)) << 4)) = make_uint4(e[4], e[5], e[6], e[7]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive_one(&raw_empty[raw]);
+      if (++raw == RAW) raw = 0, raw_phase ^= 1;
+      fence_async_shared();
+      mbar_arrive_one(&kv_full[r]);
+      if (++r == RING) r = 0, phase ^= 1;
+    };
+    for (int u = -1; u < units && ok; ++u) {
+      if (u + 1 < units) turn(std::false_type(), u + 1);
+      if (u >= 0 && ok) turn(std::true_type(), u);
     }
   } else {
     // ---- scores to weights: a thread a row
     regs_more<REGS_MANY>();
     const int t = (warp - 8) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
-    const int mine = t == 0 ? (units0 + 1) / 2 : (units1 + 1) / 2, n_tok = t == 0 ? n_tok0 : n_tok1;
+    const int mine = t == 0 ? units0 : units1, n_tok = t == 0 ? n_tok0 : n_tok1;
     const int first_pos = pos0 + t * tok, last_pos = first_pos + n_tok - 1, pos = first_pos + row / group;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const uint32_t tm_s = tmem + t * KEYS + lanes, tm_o = tmem + L::TM_O + t * 128 + lanes;
-    // whether every row of the slot sees every key of a page
-    auto whole = [&](int page) {
-      return page * PAGE + PAGE - 1 <= first_pos && (a.window == 0 || page * PAGE > last_pos - a.window || page * PAGE + PAGE <= a.keep_first);
-    };
+    const uint32_t tm_s = tmem + t * 128 + lanes, tm_o = tmem + L::TM_O + t * 128 + lanes;
     float row_mul = 1.f;
     if (mine > 0) {                                              // the row's queries to half precision, in place
       ok = mbar_wait(q_full, 0);
@@ -373,7 +360,7 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
       uint32_t top = 0;
 #pragma unroll
       for (int c = 0; c < HD / 8; ++c) {
-        x[c] = *reinterpret_cast<const uint4*>(q + (c >> 3) * L::BLOCK + (((c & 7) ^ (row & 7)) << 4));
+        x[c] = *reinterpret_cast<const uint4*>(q + (c >> 3) * Q_BLOCK + (((c & 7) ^ (row & 7)) << 4));
         top = __vmaxu2(top, __vmaxu2(__vmaxu2(x[c].x & 0x7fff7fffu, x[c].y & 0x7fff7fffu), __vmaxu2(x[c].z & 0x7fff7fffu, x[c].w & 0x7fff7fffu)));
       }
       const uint32_t e = max(top & 0xffffu, top >> 16) >> 7;     // its largest exponent
@@ -385,51 +372,47 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
         uint32_t w[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
 #pragma unroll
         for (int y = 0; y < 4; ++y) w[y] = f16_pair(__uint_as_float(w[y] << 16) * f, __uint_as_float(w[y] & 0xffff0000u) * f);
-        *reinterpret_cast<uint4*>(q + (c >> 3) * L::BLOCK + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4*>(q + (c >> 3) * Q_BLOCK + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
       }
       fence_async_shared();
       mbar_arrive_one(&q_ready[t]);
     }
     float ref = -INFINITY, sum = 0.f;            // what the weights are relative to: the row's largest t + c, or up to RISE less
     for (int i = 0; i < mine && ok; ++i) {
-      const int page0 = page_of(2 * i), page1 = 2 * i + 1 < units ? page_of(2 * i + 1) : 1 << 24;      // (no second page: keys that nobody sees)
-      const uint8_t* set = sets + (i % SCALE_SETS) * L::SET;
-      if (!mbar_wait(&s_full[t], i & 1)) { ok = false; break; }
+      const int page = page_of(i), b = i & 1;
+      const uint8_t* set = sets + (i % SETS) * L::SET;
+      if (!mbar_wait(&s_full[t * 2 + b], (i >> 1) & 1)) { ok = false; break; }
       tc_fence_after();
-      const float4 about0 = reinterpret_cast<const float4*>(set)[0], about1 = reinterpret_cast<const float4*>(set)[1];
-      const float mul0 = fmaxf(about0.x * row_mul, 0x1p-126f), mul1 = fmaxf(about1.x * row_mul, 0x1p-126f);
-      const bool marked = about0.w + about1.w > 0.f;
-      const bool look = marked || !(whole(page0) && 2 * i + 1 < units && whole(page1));
-      // The row's scores of a page.  They are read twice, for the maximum and for the weights: 128 of them do not fit a thread's registers beside what else it needs.
-      auto scores = [&](int h, uint32_t (&x)[PAGE]) {
-        tmem_ld32(tm_s + h * PAGE, x);
-        tmem_ld32(tm_s + h * PAGE + 32, x + 32);
-        tmem_ld_wait();
-        if (look) {
-          const float* mark = reinterpret_cast<const float*>(set + 32) + h * PAGE;
-          const int key0 = (h ? page1 : page0) * PAGE;
+      uint32_t x[PAGE];                          // the row's scores
+      tmem_ld32(tm_s + b * PAGE, x);
+      tmem_ld32(tm_s + b * PAGE + 32, x + 32);
+      const float4 about = *reinterpret_cast<const float4*>(set);
+      const float mul = fmaxf(about.x * row_mul, 0x1p-126f);
+      tmem_ld_wait();
+      const int last = pos - page * PAGE;        // the last key of the page that the row sees
+      if (page * PAGE + PAGE - 1 > first_pos) {
 #pragma unroll
-          for (int c = 0; c < PAGE; ++c) {
-            const int key = key0 + c;
-            const bool sees = key <= pos && (a.window == 0 || pos - key < a.window || key < a.keep_first);
-            x[c] = sees ? __float_as_uint(__uint_as_float(x[c]) + mark[c]) : 0xff800000u;
-          }
-        }
-      };
-      float top[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t x[PAGE];
-        scores(h, x);
-        float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < PAGE; c += 2) m[(c >> 1) & 3] = fmaxf(fmaxf(m[(c >> 1) & 3], __uint_as_float(x[c])), __uint_as_float(x[c + 1]));
-        top[h] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+        for (int c = 0; c < PAGE; ++c) x[c] = c <= last ? x[c] : 0xff800000u;
       }
-      const float peak = fmaxf(fmaf(top[0], mul0, about0.y), fmaf(top[1], mul1, about1.y));
+      if (a.window > 0 && page * PAGE <= last_pos - a.window && page * PAGE + PAGE > a.keep_first) {
+        const int begin = last - a.window, end = a.keep_first - page * PAGE;
+#pragma unroll
+        for (int c = 0; c < PAGE; ++c) x[c] = c > begin || c < end ? x[c] : 0xff800000u;
+      }
+      if (about.w > 0.f) {
+        const float* mark = reinterpret_cast<const float*>(set + 16);
+#pragma unroll
+        for (int c = 0; c < PAGE; ++c) x[c] = x[c] == 0xff800000u ? x[c] : __float_as_uint(__uint_as_float(x[c]) + mark[c]);
+      }
+      float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < PAGE; c += 2) m[(c >> 1) & 3] = fmaxf(fmaxf(m[(c >> 1) & 3], __uint_as_float(x[c])), __uint_as_float(x[c + 1]));
+      const float peak = fmaf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), mul, about.y);
       if (i == 0) {
         ref = peak;
-      } else if (__any_sync(0xffffffffu, peak > ref + RISE)) {   // (S of this step was begun after P V of the last had ended: the output is at rest)
+      } else if (__any_sync(0xffffffffu, peak > ref + RISE)) {
+        if (!mbar_wait(&t_full[t], (i - 1) & 1)) { ok = false; break; }      // the output is at rest
+        tc_fence_after();
         const float to = fmaxf(ref, peak), keep = ref == -INFINITY ? 0.f : exp2_fast(ref - to);
         sum *= keep;
         ref = to;
@@ -445,33 +428,28 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
         }
       }
       const float base = HEAD - (ref == -INFINITY ? 0.f : ref);  // (a row that has seen nothing yet)
+      const uint64_t mul2 = pair(mul, mul), add = pair(about.y + base, about.y + base);
+      uint64_t part[2] = {0, 0};
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint64_t mul = h ? pair(mul1, mul1) : pair(mul0, mul0), add = h ? pair(about1.y + base, about1.y + base) : pair(about0.y + base, about0.y + base);
-        uint64_t part[2] = {0, 0};
-        uint32_t x[PAGE];
-        scores(h, x);
+      for (int c0 = 0; c0 < PAGE; c0 += 16) {
+        uint32_t w[8];
 #pragma unroll
-        for (int c0 = 0; c0 < PAGE; c0 += 16) {
-          uint32_t w[8];
-#pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            float p, q;
-            halves(fma2(pair(__uint_as_float(x[c0 + 2 * c]), __uint_as_float(x[c0 + 2 * c + 1])), mul, add), p, q);
-            p = exp2_fast(p);
-            q = exp2_fast(q);
-            part[c & 1] = add2(part[c & 1], pair(p, q));
-            w[c] = f16_pair(p, q);
-          }
-          tmem_st8(tm_s + (h * PAGE + c0) / 2, w);      // (over scores that have been read: the second page's begin at column 64)
+        for (int c = 0; c < 8; ++c) {
+          float p, q;
+          halves(fma2(pair(__uint_as_float(x[c0 + 2 * c]), __uint_as_float(x[c0 + 2 * c + 1])), mul2, add), p, q);
+          p = exp2_fast(p);
+          q = exp2_fast(q);
+          part[c & 1] = add2(part[c & 1], pair(p, q));
+          w[c] = f16_pair(p, q);
         }
-        float u, v;
-        halves(add2(part[0], part[1]), u, v);
-        sum = fmaf(u + v, h ? about1.z : about0.z, sum);
+        tmem_st8(tm_s + b * PAGE + c0 / 2, w);
       }
+      float u, v;
+      halves(add2(part[0], part[1]), u, v);
+      sum = fmaf(u + v, about.z, sum);
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive_one(&p_full[t]);
+      mbar_arrive_one(&p_full[t * 2 + b]);
     }
     if (ok && mine > 0) {
       ok = mbar_wait(&t_full[t], (mine - 1) & 1);
