@@ -18,8 +18,9 @@
 //   1, 2    issue the products of a slot each: S = Q K^T of the next page (128 x 64, two places in turn) before T += P V of this one (P in tensor memory, over its
 //           S's own columns), so that a row's thread finds the next scores there when it is done with these.  (Steps of 128 keys with one place for S read Q
 //           half as often, but every step then waits for two products there and back: 7800 cycles for 128 keys of 256 rows.)
-//   4-7     turn codes to half precision in the layout the products read (128-byte swizzle), once for both slots' 256 rows: a code's byte under 0x64 is 1024 + code + 128
-//   8-11, 12-15  a thread a row: scores to weights.  The running output stays in tensor memory; it is scaled down only when a row's maximum has risen by
+//   4-11    turn codes to half precision in the layout the products read (128-byte swizzle), once for both slots' 256 rows: a code's byte under 0x64 is 1024 + code + 128;
+//           four warps the keys, four the values
+//   12-15, 16-19  a thread a row: scores to weights.  The running output stays in tensor memory; it is scaled down only when a row's maximum has risen by
 //           more than 2^8 since the last time, which after the first steps is hardly ever
 //
 // Keys a row does not see weigh nothing; scales beyond the sequence's end are taken for zero, whatever they are.  A value whose scale is not finite is a value of zeros for the
@@ -35,8 +36,9 @@ KVAD_DEFINE_LAST_ERROR()
 
 namespace {
 
-constexpr int THREADS = 512;
-constexpr int REGS_FEW = 80, REGS_TURN = 96, REGS_MANY = 168;       // of 128 a thread at launch: 80 + 96 + 2 * 168 = 4 * 128
+constexpr int THREADS = 640;
+constexpr int REGS = 96;
+constexpr int REGS_FEW = 48, REGS_TURN = 64, REGS_MANY = 152;        // of 96 a thread at launch: 48 + 2 * 64 + 2 * 152 = 5 * 96
 constexpr int SETS = 8;
 constexpr float RISE = 8.f, HEAD = 6.f;      // weights are at most 2^(RISE + HEAD)
 constexpr float SHIFT = 256.f;                  // largest scaled code: below 127 * 2 * 2^8, under half precision's 65504
@@ -266,25 +268,25 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
         }
       }
     }
-  } else if (warp < 8) {
+  } else if (warp < 12) {
     // ---- codes to half precision
     regs_fewer<REGS_TURN>();
-    const int tid = threadIdx.x - 128;
-    int raw = 0, r = 0, exponent = -64, before = -64;            // of values of the latest page and the one before (a page of zeros takes the one before's)
-    uint32_t raw_phase = 0, phase = 1;
+    const int tid = (threadIdx.x - 128) & 127;
+    int exponent = -64;                                          // of the values of the page (a page of zeros takes that of the one before)
     auto turn = [&](auto which, int u) {                         // keys or values of page u
       constexpr bool VALUES = decltype(which)::value;
-      if (!mbar_wait(&kv_empty[r], phase) || !mbar_wait(&raw_full[raw], raw_phase)) { ok = false; return; }
+      const int n = VALUES ? (u == units - 1 ? 2 * units - 1 : 2 * u + 2) : max(0, 2 * u - 1);      // its place in the order of use
+      const int r = n % RING, raw = n % RAW;
+      if (!mbar_wait(&kv_empty[r], ((n / RING) & 1) ^ 1) || !mbar_wait(&raw_full[raw], (n / RAW) & 1)) { ok = false; return; }
       uint8_t* dst = kv_tiles + r * L::KV_BYTES;
       const uint8_t* src = raw_tiles + raw * L::RAW_BYTES;
       const float* vs = reinterpret_cast<const float*>(src + L::CODES);
       const float* ks = vs + PAGE;
       const int there = min(PAGE, kv_len - page_of(u) * PAGE);   // beyond the sequence's end a scale may be anything
-      float shift;
+      const float v0 = lane < there ? vs[lane] : 0.f, v1 = lane + 32 < there ? vs[lane + 32] : 0.f;
+      exponent = top_exponent(v0, v1, exponent);
+      float shift = power_of_2(-exponent);
       if (!VALUES) {
-        const float v0 = lane < there ? vs[lane] : 0.f, v1 = lane + 32 < there ? vs[lane + 32] : 0.f;
-        before = exponent;
-        exponent = top_exponent(v0, v1, exponent);
         const int e = top_exponent(lane < there ? ks[lane] * a.scale_log2 : 0.f, lane + 32 < there ? ks[lane + 32] * a.scale_log2 : 0.f, 0);
         shift = power_of_2(-e);
         const bool b0 = !(fabsf(v0) < INFINITY), b1 = !(fabsf(v1) < INFINITY), bad = __any_sync(0xffffffffu, b0 || b1);
@@ -295,59 +297,66 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
           mark[lane + 32] = b1 ? __uint_as_float(0x7fffffffu) : 0.f;
           if (lane == 0) *reinterpret_cast<float4*>(set) = make_float4(power_of_2(e) / SHIFT, (float)exponent, power_of_2(-exponent), bad ? 1.f : 0.f);
         }
-      } else {
-        shift = power_of_2(u == units - 1 ? -exponent : -before);
       }
       constexpr int PER_ROW = HD / 16, PIECES = PAGE * PER_ROW;
       // a thread takes 16 codes; threads are dealt out so that eight neighbours read 128 bytes in a row and write pieces that lie in eight different banks' columns
+      // (all of a thread's pieces are read before the first is written: the compiler may not read past a write that might be to the same place)
+      constexpr int N = (PIECES + 127) / 128;
+      int row[N], col[N];
+      int4 codes[N];
+      float scale[N];
 #pragma unroll
-      for (int p0 = 0; p0 < PIECES; p0 += 128) {
-        const int p = p0 + tid;
+      for (int y = 0; y < N; ++y) {
+        const int p = y * 128 + tid;
+        if (PER_ROW == 8) {
+          const int q = (p >> 2) & 3;
+          row[y] = (p >> 4) * 2 + (q & 1);
+          col[y] = (p & 3) + ((q == 1 || q == 2) ? 4 : 0);
+        } else {
+          row[y] = p / PER_ROW;
+          col[y] = p - row[y] * PER_ROW;
+        }
         if (PIECES % 128 == 0 || p < PIECES) {
-          int row, c;
-          if (PER_ROW == 8) {
-            const int q = (p >> 2) & 3;
-            row = (p >> 4) * 2 + (q & 1);
-            c = (p & 3) + ((q == 1 || q == 2) ? 4 : 0);
-          } else {
-            row = p / PER_ROW;
-            c = p - row * PER_ROW;
-          }
-          const int4 w = *reinterpret_cast<const int4*>(src + row * HD + c * 16);
-          const uint32_t word[4] = {(uint32_t)w.x, (uint32_t)w.y, (uint32_t)w.z, (uint32_t)w.w};
-          float f = row < there ? (VALUES ? vs[row] : ks[row] * a.scale_log2) * shift * SHIFT : 0.f;
+          codes[y] = *reinterpret_cast<const int4*>(src + row[y] * HD + col[y] * 16);
+          scale[y] = VALUES ? vs[row[y]] : ks[row[y]];
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive_one(&raw_empty[raw]);
+      const float by = VALUES ? shift : shift * a.scale_log2;
+#pragma unroll
+      for (int y = 0; y < N; ++y) {
+        if (PIECES % 128 == 0 || y * 128 + tid < PIECES) {
+          const uint32_t word[4] = {(uint32_t)codes[y].x, (uint32_t)codes[y].y, (uint32_t)codes[y].z, (uint32_t)codes[y].w};
+          float f = row[y] < there ? scale[y] * by * SHIFT : 0.f;
           if (VALUES && !(fabsf(f) < INFINITY)) f = 0.f;         // (its weight says so)
           const __half2 hi = __float2half2_rn(f);
           const __half2 lo = __float2half2_rn(f - __low2float(hi));
           uint32_t e[8];
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
+          for (int z = 0; z < 4; ++z) {
             __half2 m, n;
-            codes_to_f16(word[y], m, n);
-            e[2 * y] = as_bits(VALUES ? __hmul2(m, hi) : __hfma2(m, hi, __hmul2(m, lo)));
-            e[2 * y + 1] = as_bits(VALUES ? __hmul2(n, hi) : __hfma2(n, hi, __hmul2(n, lo)));
+            codes_to_f16(word[z], m, n);
+            e[2 * z] = as_bits(VALUES ? __hmul2(m, hi) : __hfma2(m, hi, __hmul2(m, lo)));
+            e[2 * z + 1] = as_bits(VALUES ? __hmul2(n, hi) : __hfma2(n, hi, __hmul2(n, lo)));
           }
-          const int piece = (c & 3) * 2;
-          uint8_t* d = dst + (c >> 2) * PAGE_BLOCK + row * 128;
-          *reinterpret_cast<uint4*>(d + ((piece ^ (row & 7)) << 4)) = make_uint4(e[0], e[1], e[2], e[3]);
-          *reinterpret_cast<uint4*>(d + (((piece + 1) ^ (row & 7)) << 4)) = make_uint4(e[4], e[5], e[6], e[7]);
+          const int piece = (col[y] & 3) * 2;
+          uint8_t* d = dst + (col[y] >> 2) * PAGE_BLOCK + row[y] * 128;
+          *reinterpret_cast<uint4*>(d + ((piece ^ (row[y] & 7)) << 4)) = make_uint4(e[0], e[1], e[2], e[3]);
+          *reinterpret_cast<uint4*>(d + (((piece + 1) ^ (row[y] & 7)) << 4)) = make_uint4(e[4], e[5], e[6], e[7]);
         }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive_one(&raw_empty[raw]);
-      if (++raw == RAW) raw = 0, raw_phase ^= 1;
       fence_async_shared();
       mbar_arrive_one(&kv_full[r]);
-      if (++r == RING) r = 0, phase ^= 1;
     };
-    for (int u = -1; u < units && ok; ++u) {
-      if (u + 1 < units) turn(std::false_type(), u + 1);
-      if (u >= 0 && ok) turn(std::true_type(), u);
+    for (int u = 0; u < units && ok; ++u) {                      // keys: warps 4-7, values: 8-11
+      if (warp < 8) turn(std::false_type(), u);
+      else turn(std::true_type(), u);
     }
   } else {
     // ---- scores to weights: a thread a row
     regs_more<REGS_MANY>();
-    const int t = (warp - 8) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    const int t = (warp - 12) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const int mine = t == 0 ? units0 : units1, n_tok = t == 0 ? n_tok0 : n_tok1;
     const int first_pos = pos0 + t * tok, last_pos = first_pos + n_tok - 1, pos = first_pos + row / group;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
@@ -500,8 +509,8 @@ int launch(const void* q, int64_t ld_q, int n_rows, const Args& a, int max_new, 
   if (!configured) {
     cudaFuncAttributes attr;
     cudaError_t e = cudaFuncGetAttributes(&attr, kernel);
-    if (e == cudaSuccess && attr.numRegs != 65536 / THREADS)       // what the roles share out among themselves
-      KVAD_FAIL(KVAD_ERR_CUDA, "attention_int8_prompt: built with %d registers a thread, not %d", attr.numRegs, 65536 / THREADS);
+    if (e == cudaSuccess && attr.numRegs != REGS)       // what the roles share out among themselves
+      KVAD_FAIL(KVAD_ERR_CUDA, "attention_int8_prompt: built with %d registers a thread, not %d", attr.numRegs, REGS);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::SMEM);
     if (e != cudaSuccess) KVAD_FAIL(KVAD_ERR_CUDA, "attention_int8_prompt: cannot reserve %zu bytes of shared memory: %s", L::SMEM, cudaGetErrorString(e));
     configured = true;
