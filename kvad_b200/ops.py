@@ -224,7 +224,9 @@ _SIGNATURES = {
     },
     "attention_int8": {
         "kvad_attention_int8": [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
-                                c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p],
+                                c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
+        "kvad_attention_int8_status": [],
+        "kvad_attention_int8_test_hooks": [c_uint, c_int],
     },
     "attention_int8_prompt": {
         "kvad_attention_int8_prompt": [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -1971,10 +1973,31 @@ class Ops:
                                                 int(n_seqs), int(max_new), int(n_heads), n_kv, hd, page, float(scale), int(window or 0), int(keep_first or 0),
                                                 _stream()), h)
             return
+        splits, split_pages, warps, scratch = 1, 0, 4, None
+        if max_new == 1:
+            reach = page_table.shape[1] if not window else min(page_table.shape[1], -(-window // 64) + 1 + -(-keep_first // 64))
+            splits, split_pages, warps = self.int8_splits(n_seqs * n_kv * -(-(n_heads // n_kv) // 16), reach)
+            if splits > 1:
+                scratch = torch.empty(n * n_heads * splits * (hd + 2), dtype=torch.float32, device=q.device)
         h = lib("attention_int8")
         _check(h.kvad_attention_int8(self.code, q.data_ptr(), ld_q, out.data_ptr(), ld_o, seq_starts.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(),
-                                     page_table.shape[1], k_pages.data_ptr(), k_scales.data_ptr(), v_pages.data_ptr(), v_scales.data_ptr(), n, int(n_seqs),
-                                     int(max_new), int(n_heads), n_kv, hd, page, float(scale), int(window or 0), int(keep_first or 0), _stream()), h)
+                                     page_table.shape[1], k_pages.data_ptr(), k_scales.data_ptr(), v_pages.data_ptr(), v_scales.data_ptr(), k_pages.shape[0], n,
+                                     int(n_seqs), int(max_new), int(n_heads), n_kv, hd, page, float(scale), int(window or 0), int(keep_first or 0), splits,
+                                     split_pages, warps, _ptr(scratch), _stream()), h)
+        if splits > 1:
+            global _launches
+            _launches += 1          # the blocks of a row and head meet
+
+    @staticmethod
+    def int8_splits(items: int, reach: int, n_sms: Optional[int] = None) -> tuple:
+        """How single-token rows deal out the pages of a sequence and key/value head (`items` of them, `reach` pages each at most): (blocks, pages a block,
+        warps a block).  Up to 16 pages one block of eight warps has them all; beyond, blocks of four warps, two an SM at least where four pages (one a
+        warp) are left to each, and 16 pages a block at most, so that sequences of unequal lengths keep all SMs busy."""
+        if reach <= 16:
+            return 1, 0, 8
+        want = -(-2 * (n_sms or sm_count()) // max(1, items))
+        pages = max(4, min(16, -(-reach // want)))
+        return -(-reach // pages), pages, 4
 
     # -- sampling ------------------------------------------------------------------
     ARGMAX_CHUNK = 2048
