@@ -5,14 +5,16 @@
 //
 // j over the positions that i sees: j <= i, and with a window i - j < window or j < keep_first.
 //
-// A block has up to 16 rows - (token, head) pairs of one key/value head's group: the heads of a single token, or of a few - and a range of pages; its warps
+// A block has 8 or 16 rows - (token, head) pairs of one key/value head's group: the heads of a single token, or of a few - and a range of pages; its warps
 // take the pages in turn, each with its own running maximum, sums and outputs, and they meet in shared memory at the end (and blocks of the same rows in
 // `scratch`, which a second kernel reads).  Single tokens are bound by the bytes of the cache: every warp has a page of keys and one of values on their way
 // (TMA, swizzled by their row's length) while it works on those before, so an SM has some 100 KB in flight.
 //
-// The products run on mma.sync in half precision with codes as they are (whole numbers, exact): a byte under 0x64 is 1024 + code + 128, less 1152.  A
-// row's queries are brought to [1, 4) by a power of two, exactly, and in 32-bit go in two pieces (22 bits); the scales come in on the scores, which a thread has for two
-// keys of eight.  Weights times their value's scale go in as half precision in one piece (11 bits; the output has 8), or two.  To keep them in range the exponent c of a
+// The products run on mma.sync in half precision with codes as they are (whole numbers, exact): a byte under 0x64 is 1024 + code + 128, less 1152.  Keys, and
+// entries of values, are the 16-wide side of the product and rows the 8-wide one, S^T = K Q^T and O^T = V^T P^T: with the rows on the 16-wide side a
+// page of a head with 4 queries took twice the instructions.  A
+// row's queries are brought to [1, 4) by a power of two, exactly, and in 32-bit go in two pieces (22 bits); the scales come in on the scores, which a thread has for eight
+// keys and two rows.  Weights times their value's scale go in as half precision in one piece (11 bits; the output has 8), or two.  To keep them in range the exponent c of a
 // page's largest value scale is kept apart: with t the score in powers of two,
 //
 //   p_ij = 2^(t_ij + c - r_i + 12),   out_i = sum_j (p_ij vs_j 2^-c) vc_j / sum_j p_ij 2^-c,   r_i the largest t + c seen so far.
@@ -31,7 +33,7 @@ KVAD_DEFINE_LAST_ERROR()
 
 namespace {
 
-constexpr int PAGE = 64, ROWS = 16;
+constexpr int PAGE = 64;
 constexpr float LOG2E = 1.4426950408889634f, HEAD = 12.f;
 
 bool g_skip_copy = false;                       // tests: the next launch's warps leave out their first page
@@ -51,14 +53,14 @@ struct Args {
   float scale_log2;
 };
 
-// HDP: entries of a head, rounded up to a power of two; the rest come as zeros.
-template <int HDP, int PIECES> struct Layout {
+// HDP: entries of a head, rounded up to a power of two; the rest come as zeros.  NT: eights of rows.
+template <int HDP, int PIECES, int NT> struct Layout {
   static constexpr int PITCH = HDP < 128 ? HDP : 128, BLOCKS = (HDP + 127) / 128;      // bytes of a swizzled row; of them a key has so many
   static constexpr int KS = HDP / 16;                            // 16-entry steps
   static constexpr uint32_t TILE = PAGE * HDP;
   static constexpr uint32_t WARP = 2 * TILE + 2 * PAGE * 4;      // keys, values, their scales
   static constexpr uint32_t OFF_Q = 1024;                        // (mbarriers and the like before)
-  static constexpr uint32_t Q_BYTES = PIECES * KS * 512;
+  static constexpr uint32_t Q_BYTES = PIECES * NT * KS * 256;
   static constexpr uint32_t OFF_WARPS = (OFF_Q + Q_BYTES + 1023) / 1024 * 1024;
   static constexpr size_t smem(int warps) { return OFF_WARPS + (size_t)warps * ((WARP + 1023) / 1024 * 1024) + 1024; }
 };
@@ -81,9 +83,16 @@ __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
 __device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ void mma_f16(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+// (not volatile: the products of different accumulators may be dealt among one another)
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, const uint2& b) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y));
+}
+// An 8 x 8 matrix of 16-bit numbers, a lane two neighbours of a row, turned over.
+__device__ __forceinline__ uint32_t turned(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 // Two of a word's four codes as half precision; SEL says which.
 template <uint32_t SEL> __device__ __forceinline__ uint32_t two_codes(uint32_t offset_word) {
@@ -97,19 +106,19 @@ template <int HDP> __device__ __forceinline__ uint32_t place(int row, int c) {
   return (c >> 3) * (PAGE * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
 }
 
-template <typename T, int HDP>
+template <typename T, int HDP, int NT>
 __global__ void __launch_bounds__(256)
 attention_int8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Args a) {
   constexpr int PIECES = std::is_same<T, float>::value ? 2 : 1;
-  using L = Layout<HDP, PIECES>;
-  constexpr int KS = L::KS;
+  using L = Layout<HDP, PIECES, NT>;
+  constexpr int KS = L::KS, ROWS = 8 * NT;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, warps = blockDim.x >> 5;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem) + 2 * warp;                    // a page's keys, its values have come
   volatile int* failed = reinterpret_cast<volatile int*>(smem + 256);
   float* row_mul = reinterpret_cast<float*>(smem + 512);                           // [ROWS] what the queries were divided by
-  uint4* q_frag = reinterpret_cast<uint4*>(smem + L::OFF_Q);                       // [piece][step][lane]
+  uint2* q_frag = reinterpret_cast<uint2*>(smem + L::OFF_Q);                       // [piece][step][eight of rows][lane]
   uint8_t* mine = smem + L::OFF_WARPS + warp * ((L::WARP + 1023) / 1024 * 1024);
   uint8_t* k_tile = mine;
   uint8_t* v_tile = mine + L::TILE;
@@ -191,11 +200,10 @@ attention_int8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
       const int d = i * 32 + lane, step = d >> 4, tt = (d >> 2) & 3, e4 = d & 3;      // entry of step `step`: thread tt's, the e4-th of its four
       if (d < HDP) {
         float y = x[i] * f;
-        const int reg = (e4 >> 1) * 2 + (r >> 3);                // a0, a1: entries 0 and 1 of rows g and g + 8; a2, a3: entries 2 and 3
 #pragma unroll
-        for (int p = 0; p < PIECES; ++p) {
+        for (int p = 0; p < PIECES; ++p) {                       // (the products' order: k = 2t, 2t + 1 are entries 0 and 1 of thread t's four, 2t + 8, 2t + 9 entries 2 and 3)
           const __half h = __float2half_rn(y);
-          reinterpret_cast<__half*>(q_frag)[((size_t)(p * KS + step) * 32 + (r & 7) * 4 + tt) * 8 + reg * 2 + (e4 & 1)] = h;
+          reinterpret_cast<__half*>(q_frag)[(((p * KS + step) * NT + (r >> 3)) * 32 + (r & 7) * 4 + tt) * 4 + e4] = h;
           y -= __half2float(h);
         }
       }
@@ -203,12 +211,23 @@ attention_int8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   }
   __syncthreads();
 
-  float o[2 * KS][4];
+  float o[KS][NT][4];                             // entries 16 i + 2 g (and + 1: the last two) of rows 2 t, 2 t + 1
 #pragma unroll
-  for (int i = 0; i < 2 * KS; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  float ref[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};    // of rows g and g + 8; sums of this thread's keys
-  const int pos[2] = {pos0 + g / heads, pos0 + (g + 8) / heads};
-  const float mul[2] = {row_mul[g] * a.scale_log2, row_mul[g + 8] * a.scale_log2};
+  for (int i = 0; i < KS; ++i)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f;
+  float ref[NT][2], sum[NT][2], mul[NT][2];       // of rows 8 n + 2 t + e; sums of this thread's keys
+  int pos[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = 8 * n + 2 * t + e;
+      ref[n][e] = -INFINITY;
+      sum[n][e] = 0.f;
+      mul[n][e] = row_mul[r] * a.scale_log2;
+      pos[n][e] = pos0 + r / heads;
+    }
   int exponent = -64;
   uint32_t phase = 0;
   bool ok = true;
@@ -222,153 +241,171 @@ attention_int8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     const int next_id = __shfl_sync(0xffffffffu, id, ahead);
     const bool more = u + warps < u_end;
     const int page = page_of(u), there = kv_len - page * PAGE;
-    // ---- scores: 16 rows x 64 keys
+    const int m8 = lane >> 3;                                    // of four matrices the one whose row this lane points at
+    // ---- scores: 64 keys x rows; key 16 m + g (and + 8: the last two) of rows 2 t, 2 t + 1
     if (!mbar_wait(&bars[0], phase)) { ok = false; break; }
-    float sc[8][4];
+    float sc[4][NT][4];
 #pragma unroll
-    for (int n = 0; n < 8; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
-    constexpr int STEPS = KS < 4 ? KS : 4, TILES = 4 / STEPS;    // four matrices a load: so many steps of so many groups of eight keys
+    for (int m = 0; m < 4; ++m)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) sc[m][n][0] = sc[m][n][1] = sc[m][n][2] = sc[m][n][3] = 0.f;
+    constexpr int STEPS = KS < 2 ? 1 : 2, TILES = 2 / STEPS;     // four matrices a load: two halves of 16 keys, of two steps or of two sixteens of keys
 #pragma unroll
     for (int s0 = 0; s0 < KS; s0 += STEPS) {
-      uint4 qf[PIECES][STEPS];
+      uint32_t w[4][4];
 #pragma unroll
-      for (int p = 0; p < PIECES; ++p)
+      for (int m = 0; m < 4; m += TILES)
+        ldmatrix4(k_addr + place<HDP>((m + (STEPS == 2 ? 0 : m8 >> 1)) * 16 + (m8 & 1) * 8 + (lane & 7), s0 + (STEPS == 2 ? m8 >> 1 : 0)), w[m]);
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) qf[p][i] = q_frag[(p * KS + s0 + i) * 32 + lane];
+      for (int i = 0; i < STEPS; ++i) {
+        uint2 q[PIECES][NT];
 #pragma unroll
-      for (int n = 0; n < 8; n += TILES) {
-        uint32_t w[4];
-        const int m = lane >> 3;                                 // the matrix whose row this lane points at
-        ldmatrix4(k_addr + place<HDP>((n + m / STEPS) * 8 + (lane & 7), s0 + m % STEPS), w);
+        for (int p = 0; p < PIECES; ++p)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t x = w[i] ^ 0x80808080u, b0 = two_codes<0x4140>(x), b1 = two_codes<0x4342>(x);
+          for (int n = 0; n < NT; ++n) q[p][n] = q_frag[((p * KS + s0 + i) * NT + n) * 32 + lane];
 #pragma unroll
-          for (int p = PIECES - 1; p >= 0; --p) mma_f16(sc[n + i / STEPS], qf[p][i % STEPS], b0, b1);
+        for (int m = 0; m < 4; ++m) {
+          const uint32_t x = w[STEPS == 2 ? m : m & ~1][STEPS == 2 ? 2 * i : 2 * (m & 1)] ^ 0x80808080u;
+          const uint32_t y = w[STEPS == 2 ? m : m & ~1][STEPS == 2 ? 2 * i + 1 : 2 * (m & 1) + 1] ^ 0x80808080u;
+          const uint32_t a0 = two_codes<0x4140>(x), a1 = two_codes<0x4140>(y), a2 = two_codes<0x4342>(x), a3 = two_codes<0x4342>(y);
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int p = PIECES - 1; p >= 0; --p) mma_f16(sc[m][n], a0, a1, a2, a3, q[p][n]);
         }
       }
     }
     // scores in powers of two
-    float scale[8][2];
+    float k_by[4][2];
 #pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      const float2 k2 = *reinterpret_cast<const float2*>(ks + n * 8 + 2 * t);
-      scale[n][0] = k2.x;
-      scale[n][1] = k2.y;
+    for (int m = 0; m < 4; ++m) {
+      k_by[m][0] = ks[16 * m + g];
+      k_by[m][1] = ks[16 * m + g + 8];
     }
 #pragma unroll
-    for (int n = 0; n < 8; ++n)
+    for (int m = 0; m < 4; ++m)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sc[n][e] *= scale[n][e & 1] * mul[e >> 1];
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[m][n][e] *= k_by[m][e >> 1] * mul[n][e & 1];
     __syncwarp();
     if (lane == 0 && more) ask(false, next_id, false);           // these keys have been read
     const bool masked = page * PAGE + PAGE - 1 > pos0 || (a.window > 0 && page * PAGE <= last_pos - a.window && page * PAGE + PAGE > a.keep_first);
     if (masked) {
 #pragma unroll
-      for (int n = 0; n < 8; ++n)
+      for (int m = 0; m < 4; ++m)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int key = page * PAGE + n * 8 + 2 * t + (e & 1), p = pos[e >> 1];
-          if (!(key <= p && (a.window == 0 || p - key < a.window || key < a.keep_first))) sc[n][e] = -INFINITY;
-        }
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = page * PAGE + 16 * m + g + 8 * (e >> 1), p = pos[n][e & 1];
+            if (!(key <= p && (a.window == 0 || p - key < a.window || key < a.keep_first))) sc[m][n][e] = -INFINITY;
+          }
     }
     // ---- weights
     if (!mbar_wait(&bars[1], phase)) { ok = false; break; }
-    float vsc[8][2];
+    float v_by[4][2];
+    uint32_t top = 0;                                            // the exponent of the largest of the page's scales that is finite and the sequence's
 #pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      const float2 v2 = *reinterpret_cast<const float2*>(vs + n * 8 + 2 * t);
-      vsc[n][0] = v2.x;
-      vsc[n][1] = v2.y;
-    }
-    {
-      uint32_t top = 0;                                          // the exponent of the largest of the page's scales that is finite and the sequence's
+    for (int m = 0; m < 4; ++m)
 #pragma unroll
-      for (int n = 0; n < 8; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint32_t bits = __float_as_uint(vsc[n][e]) & 0x7fffffffu;
-          if (n * 8 + 2 * t + e < there && bits < 0x7f800000u) top = max(top, bits);
-        }
-      top = __reduce_max_sync(0xffffffffu, top) >> 23;
-      if (top > 0) exponent = (int)top - 127;                    // (a page of zeros takes that of the values before)
-    }
+      for (int e = 0; e < 2; ++e) {
+        v_by[m][e] = vs[16 * m + g + 8 * e];
+        const uint32_t bits = __float_as_uint(v_by[m][e]) & 0x7fffffffu;
+        if (16 * m + g + 8 * e < there && bits < 0x7f800000u) top = max(top, bits);
+      }
+    top = __reduce_max_sync(0xffffffffu, top) >> 23;
+    if (top > 0) exponent = (int)top - 127;                      // (a page of zeros takes that of the values before)
     const float c = (float)exponent, down = power_of_2(-exponent);
-    float keep[2];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      float m = -INFINITY;
+    for (int m = 0; m < 4; ++m) v_by[m][0] *= down, v_by[m][1] *= down;
+    float keep[NT][2];
+    bool changed = false;
 #pragma unroll
-      for (int n = 0; n < 8; ++n) m = fmaxf(m, fmaxf(sc[n][2 * r], sc[n][2 * r + 1]));
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2)) + c;
-      const float to = fmaxf(ref[r], m);
-      keep[r] = to == -INFINITY ? 1.f : exp2_fast(ref[r] - to);
-      ref[r] = to;
-      const float add = c + HEAD - (to == -INFINITY ? 0.f : to);
-      float part = 0.f;
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int n = 0; n < 8; ++n)
+      for (int e = 0; e < 2; ++e) {
+        float top_score = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float p = exp2_fast(sc[n][2 * r + e] + add);
-          part += p;
-          const float w = p * (vsc[n][e] * down);
-          sc[n][2 * r + e] = masked && sc[n][2 * r + e] == -INFINITY ? 0.f : w;      // (a scale that is not finite is for those alone who see it)
-        }
-      sum[r] = fmaf(sum[r], keep[r], part * down);
-    }
-    // ---- outputs: 64 keys x HDP.  In 32-bit a page's products have an accumulator of their own that joins the running output by a rounded addition: the tensor core
-    // truncates what it adds up, which over a long sequence would show.
+        for (int m = 0; m < 4; ++m) top_score = fmaxf(fmaxf(top_score, sc[m][n][e]), sc[m][n][e + 2]);
+#pragma unroll
+        for (int x = 4; x < 32; x *= 2) top_score = fmaxf(top_score, __shfl_xor_sync(0xffffffffu, top_score, x));
+        const float to = fmaxf(ref[n][e], top_score + c);
+        changed |= to != ref[n][e];
+        keep[n][e] = to == -INFINITY ? 1.f : exp2_fast(ref[n][e] - to);
+        ref[n][e] = to;
+        const float add = c + HEAD - (to == -INFINITY ? 0.f : to);
+        float part = 0.f;
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float p = exp2_fast(sc[m][n][e + 2 * h] + add);
+            part += p;
+            const float w = p * v_by[m][h];
+            sc[m][n][e + 2 * h] = masked && sc[m][n][e + 2 * h] == -INFINITY ? 0.f : w;      // (a scale that is not finite is for those alone who see it)
+          }
+        sum[n][e] = fmaf(sum[n][e], keep[n][e], part * down);
+      }
+    // ---- outputs: HDP entries x rows.  In 32-bit a page's products have an accumulator of their own that joins the running output by a rounded addition: the
+    // tensor core truncates what it adds up, which over a long sequence would show.
     constexpr bool APART = PIECES == 2;
-    if (!APART && __any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
+    if (!APART && __any_sync(0xffffffffu, changed)) {
 #pragma unroll
-      for (int i = 0; i < 2 * KS; ++i)
+      for (int i = 0; i < KS; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][e] *= keep[e >> 1];
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i][n][e] *= keep[n][e & 1];
     }
-    uint4 pf[PIECES][4];                                         // of 16 keys each
+    uint2 pf[PIECES][4][NT];                                     // of 16 keys each: a row a lane's g, its keys 2 t, 2 t + 1 and 8 further on
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {                              // a0, a1: eight keys of rows g and g + 8; a2, a3: the next eight
-        float x = sc[2 * j + (i >> 1)][(i & 1) * 2], y = sc[2 * j + (i >> 1)][(i & 1) * 2 + 1];
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int p = 0; p < PIECES; ++p) {
-          const __half2 h = __floats2half2_rn(x, y);
-          (i == 0 ? pf[p][j].x : i == 1 ? pf[p][j].y : i == 2 ? pf[p][j].z : pf[p][j].w) = as_bits(h);
-          x -= __low2float(h);
-          y -= __high2float(h);
-        }
-      }
+        for (int h = 0; h < 2; ++h) {
+          float x = sc[j][n][2 * h], y = sc[j][n][2 * h + 1];
 #pragma unroll
-    for (int c0 = 0; c0 < KS; c0 += 2) {                         // two pieces of 16 entries (one where a head has no more)
-      constexpr int NC = KS == 1 ? 1 : 2;
-      float fresh[2 * NC][4];
-#pragma unroll
-      for (int i = 0; i < 2 * NC; ++i) fresh[i][0] = fresh[i][1] = fresh[i][2] = fresh[i][3] = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t w[4];
-        const int m = lane >> 3, col = KS == 1 ? 0 : c0 + (m >> 1);
-        ldmatrix4_trans(v_addr + place<HDP>(j * 16 + (m & 1) * 8 + (lane & 7), col), w);
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-          const uint32_t x = w[2 * i] ^ 0x80808080u, y = w[2 * i + 1] ^ 0x80808080u;
-          const uint32_t e0 = two_codes<0x4240>(x), e1 = two_codes<0x4240>(y), d0 = two_codes<0x4341>(x), d1 = two_codes<0x4341>(y);
-#pragma unroll
-          for (int p = PIECES - 1; p >= 0; --p) {
-            mma_f16(APART ? fresh[2 * i] : o[2 * (c0 + i)], pf[p][j], e0, e1);                      // entries 2g of the sixteen
-            mma_f16(APART ? fresh[2 * i + 1] : o[2 * (c0 + i) + 1], pf[p][j], d0, d1);              // entries 2g + 1
+          for (int p = 0; p < PIECES; ++p) {
+            const __half2 z = __floats2half2_rn(x, y);
+            (h ? pf[p][j][n].y : pf[p][j][n].x) = turned(as_bits(z));
+            x -= __low2float(z);
+            y -= __high2float(z);
           }
         }
-      }
-      if (APART) {
+    constexpr int NC = KS == 1 ? 1 : 2;                          // sixteens of entries a load
+    auto values = [&](int j, int c0, float (&acc)[NC][NT][4]) {
+      uint32_t w[4];
+      ldmatrix4_trans(v_addr + place<HDP>(j * 16 + (m8 & 1) * 8 + (lane & 7), KS == 1 ? 0 : c0 + (m8 >> 1)), w);
 #pragma unroll
-        for (int i = 0; i < 2 * NC; ++i)
+      for (int i = 0; i < NC; ++i) {
+        const uint32_t x = w[2 * i] ^ 0x80808080u, y = w[2 * i + 1] ^ 0x80808080u;
+        const uint32_t a0 = two_codes<0x4240>(x), a1 = two_codes<0x4341>(x), a2 = two_codes<0x4240>(y), a3 = two_codes<0x4341>(y);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[2 * c0 + i][e] = fmaf(o[2 * c0 + i][e], keep[e >> 1], fresh[i][e]);
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int p = PIECES - 1; p >= 0; --p) mma_f16(acc[i][n], a0, a1, a2, a3, pf[p][j][n]);
       }
+    };
+    if (APART) {
+#pragma unroll
+      for (int c0 = 0; c0 < KS; c0 += NC) {
+        float fresh[NC][NT][4] = {};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) values(j, c0, fresh);
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[c0 + i][n][e] = fmaf(o[c0 + i][n][e], keep[n][e & 1], fresh[i][n][e]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int c0 = 0; c0 < KS; c0 += NC) values(j, c0, reinterpret_cast<float(&)[NC][NT][4]>(o[c0]));
     }
     __syncwarp();
     if (lane == 0 && more) ask(true, next_id, false);            // these values have been read
@@ -376,27 +413,25 @@ attention_int8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   if (!ok) *failed = 1;
 
   // ---- the warps meet: outputs in the keys' place, maxima and sums in the scales'
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
-    sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
-  }
+  constexpr int TURN = HDP / 2 - 1;               // (pairs of entries are turned by the row against bank conflicts)
   const bool worked = u_begin + warp < u_end;
-  if (worked && ok) {
-    float4* dst = reinterpret_cast<float4*>(k_tile);             // [ROWS][HDP], four entries at a time, turned by the row against bank conflicts
 #pragma unroll
-    for (int i = 0; i < KS; ++i)
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int r = 0; r < 2; ++r)                                // entries 16 i + 4 t ..: 2 (2t) + {0, 1}, 2 (2t + 1) + {0, 1}
-        dst[(g + 8 * r) * (HDP / 4) + ((4 * i + t) ^ (g & (HDP / 4 < 8 ? HDP / 4 - 1 : 7)))] =
-            make_float4(o[2 * i][2 * r], o[2 * i + 1][2 * r], o[2 * i][2 * r + 1], o[2 * i + 1][2 * r + 1]);
-  }
-  if (t == 0) {
-    ks[g] = worked ? ref[0] : -INFINITY;
-    ks[g + 8] = worked ? ref[1] : -INFINITY;
-    vs[g] = sum[0];
-    vs[g + 8] = sum[1];
-  }
+    for (int e = 0; e < 2; ++e) {
+      const int r = 8 * n + 2 * t + e;
+#pragma unroll
+      for (int x = 4; x < 32; x *= 2) sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], x);
+      if (worked && ok) {
+        float2* dst = reinterpret_cast<float2*>(k_tile);         // [ROWS][HDP]
+#pragma unroll
+        for (int i = 0; i < KS; ++i) dst[r * (HDP / 2) + ((8 * i + g) ^ (((r & 6) * 4) & TURN))] = make_float2(o[i][n][e], o[i][n][e + 2]);
+      }
+      if (g == 0) {
+        ks[r] = worked ? ref[n][e] : -INFINITY;
+        vs[r] = sum[n][e];
+      }
+    }
   __syncthreads();
   if (*failed) {
     outlast_what_is_in_flight();
@@ -405,28 +440,30 @@ attention_int8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   const int busy = max(0, min(warps, u_end - u_begin));
   const size_t stride = (L::WARP + 1023) / 1024 * 1024;
   const uint8_t* base = smem + L::OFF_WARPS;
-  for (int i = threadIdx.x; i < ROWS * (HDP / 4); i += blockDim.x) {
-    const int r = i / (HDP / 4), d4 = i - r * (HDP / 4), token = r / heads, head = r - token * heads;
-    if (token >= n_tok || head >= n_heads || d4 * 4 >= a.hd) continue;
+  for (int i = threadIdx.x; i < ROWS * (HDP / 2); i += blockDim.x) {
+    const int r = i / (HDP / 2), d2 = i - r * (HDP / 2), token = r / heads, head = r - token * heads;
+    if (token >= n_tok || head >= n_heads || d2 * 2 >= a.hd) continue;
     float top = -INFINITY, l = 0.f;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    float2 x = make_float2(0.f, 0.f);
     for (int w = 0; w < busy; ++w) top = fmaxf(top, reinterpret_cast<const float*>(base + w * stride + 2 * L::TILE)[r]);
     for (int w = 0; w < busy; ++w) {
       const float* m = reinterpret_cast<const float*>(base + w * stride + 2 * L::TILE);
       const float f = m[r] == -INFINITY ? 0.f : exp2_fast(m[r] - top);
-      const float4 y = reinterpret_cast<const float4*>(base + w * stride)[r * (HDP / 4) + (d4 ^ (r & (HDP / 4 < 8 ? HDP / 4 - 1 : 7)))];
+      const float2 y = reinterpret_cast<const float2*>(base + w * stride)[r * (HDP / 2) + (d2 ^ (((r & 6) * 4) & TURN))];
       l = fmaf(m[PAGE + r], f, l);
-      x.x = fmaf(y.x, f, x.x); x.y = fmaf(y.y, f, x.y); x.z = fmaf(y.z, f, x.z); x.w = fmaf(y.w, f, x.w);
+      x.x = fmaf(y.x, f, x.x);
+      x.y = fmaf(y.y, f, x.y);
     }
     const int64_t row = row0 + tile * tok + token;
     if (a.splits > 1) {
       float* dst = a.scratch + ((row * a.n_heads + h0 + head) * a.splits + split) * (a.hd + 2);
-      if (d4 == 0) dst[a.hd] = top, dst[a.hd + 1] = l;
-      if (busy > 0) dst[d4 * 4] = x.x, dst[d4 * 4 + 1] = x.y, dst[d4 * 4 + 2] = x.z, dst[d4 * 4 + 3] = x.w;
+      if (d2 == 0) dst[a.hd] = top, dst[a.hd + 1] = l;
+      if (busy > 0) dst[d2 * 2] = x.x, dst[d2 * 2 + 1] = x.y;
     } else {
-      T* dst = reinterpret_cast<T*>(a.out) + row * a.ld_out + (int64_t)(h0 + head) * a.hd + d4 * 4;
+      T* dst = reinterpret_cast<T*>(a.out) + row * a.ld_out + (int64_t)(h0 + head) * a.hd + d2 * 2;
       const float inv = 1.f / l;
-      dst[0] = from_f32<T>(x.x * inv); dst[1] = from_f32<T>(x.y * inv); dst[2] = from_f32<T>(x.z * inv); dst[3] = from_f32<T>(x.w * inv);
+      dst[0] = from_f32<T>(x.x * inv);
+      dst[1] = from_f32<T>(x.y * inv);
     }
   }
 }
@@ -474,15 +511,16 @@ int tensor_map(const int8_t* p, int64_t rows, int hd, int pitch, CUtensorMap* ma
   return KVAD_OK;
 }
 
-template <typename T, int HDP>
+template <typename T, int HDP, int NT>
 int launch(const Args& a, const int8_t* k, const int8_t* v, int64_t cache_rows, int max_new, int warps, cudaStream_t stream) {
   constexpr int PIECES = std::is_same<T, float>::value ? 2 : 1;
-  using L = Layout<HDP, PIECES>;
+  using L = Layout<HDP, PIECES, NT>;
+  constexpr int ROWS = 8 * NT;
   CUtensorMap mk, mv;
   int rc = tensor_map(k, cache_rows, a.hd, L::PITCH, &mk);
   if (rc == KVAD_OK) rc = tensor_map(v, cache_rows, a.hd, L::PITCH, &mv);
   if (rc != KVAD_OK) return rc;
-  auto kernel = attention_int8_kernel<T, HDP>;
+  auto kernel = attention_int8_kernel<T, HDP, NT>;
   while (warps > 1 && L::smem(warps) > 227 * 1024) warps /= 2;
   static bool configured = false;
   if (!configured) {
@@ -500,9 +538,14 @@ int launch(const Args& a, const int8_t* k, const int8_t* v, int64_t cache_rows, 
 
 template <typename T>
 int by_size(const Args& a, const int8_t* k, const int8_t* v, int64_t cache_rows, int n_rows, int max_new, int warps, cudaStream_t stream) {
-  const int rc = a.hd <= 16 ? launch<T, 16>(a, k, v, cache_rows, max_new, warps, stream) : a.hd <= 32 ? launch<T, 32>(a, k, v, cache_rows, max_new, warps, stream)
-                 : a.hd <= 64 ? launch<T, 64>(a, k, v, cache_rows, max_new, warps, stream) : a.hd <= 128 ? launch<T, 128>(a, k, v, cache_rows, max_new, warps, stream)
-                                                                                             : launch<T, 256>(a, k, v, cache_rows, max_new, warps, stream);
+  const int group = a.n_heads / a.kv_heads;
+  const bool few = max_new == 1 && group <= 8;   // (more rows share what it takes to bring and turn the codes, where there are more)
+  auto go = [&](auto size) {
+    constexpr int HDP = decltype(size)::value;
+    return few ? launch<T, HDP, 1>(a, k, v, cache_rows, max_new, warps, stream) : launch<T, HDP, 2>(a, k, v, cache_rows, max_new, warps, stream);
+  };
+  const int rc = a.hd <= 16 ? go(std::integral_constant<int, 16>()) : a.hd <= 32 ? go(std::integral_constant<int, 32>())
+                 : a.hd <= 64 ? go(std::integral_constant<int, 64>()) : a.hd <= 128 ? go(std::integral_constant<int, 128>()) : go(std::integral_constant<int, 256>());
   if (rc != KVAD_OK || a.splits == 1) return rc;
   const int64_t blocks = ((int64_t)n_rows * a.n_heads + 3) / 4;
   KVAD_REQUIRE(blocks < (1ll << 31), "attention_int8: more rows and heads than a launch takes");
