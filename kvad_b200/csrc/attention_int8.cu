@@ -107,7 +107,7 @@ template <int HDP> __device__ __forceinline__ uint32_t place(int row, int c) {
 }
 
 template <typename T, int HDP, int NT>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, (NT == 1 && HDP <= 64 ? 3 : NT == 1 && HDP <= 128 ? 2 : 1))
 attention_int8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Args a) {
   constexpr int PIECES = std::is_same<T, float>::value ? 2 : 1;
   using L = Layout<HDP, PIECES, NT>;
@@ -135,17 +135,20 @@ attention_int8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   rest -= s * a.kv_heads * chunks;
   const int kvh = rest / chunks, h0 = kvh * group + (rest - kvh * chunks) * heads, n_heads = min(heads, (kvh + 1) * group - h0);
   pdl_wait();
-  const int row0 = a.seq_starts[s], n_new = a.seq_starts[s + 1] - row0;
+  // (what does not wait for another number from memory is asked for together: without a window the pages' numbers too)
+  const int* pages = a.table + (int64_t)s * a.table_width;
+  const int begin = split * a.split_pages + warp;
+  int id = a.window == 0 && begin + lane * warps < a.table_width ? pages[begin + lane * warps] : 0;      // a lane has the number of every 32nd page of this warp's
+  const int row0 = a.seq_starts[s], row1 = a.seq_starts[s + 1], kv_len = a.kv_lens[s], n_new = row1 - row0;
   const int tile = (n_new + tok - 1) / tok - 1 - from_end;
   if (tile < 0) return;
-  const int kv_len = a.kv_lens[s], n_tok = min(tok, n_new - tile * tok);
+  const int n_tok = min(tok, n_new - tile * tok);
   const int pos0 = kv_len - n_new + tile * tok, last_pos = pos0 + n_tok - 1;
   const int first_page = a.window > 0 ? max(0, pos0 - a.window + 1) / PAGE : 0;
   const int kept = min((a.keep_first + PAGE - 1) / PAGE, first_page);
   const int units = kept + last_pos / PAGE - first_page + 1;
   auto page_of = [&](int u) { return u < kept ? u : first_page + u - kept; };
   const int u_begin = split * a.split_pages, u_end = a.splits > 1 ? min(units, u_begin + a.split_pages) : units;
-  const int* pages = a.table + (int64_t)s * a.table_width;
 
   if (threadIdx.x == 0) {
     prefetch_tensormap(&map_k);
@@ -160,10 +163,9 @@ attention_int8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   }
   __syncwarp();
 
-  // a lane has the number of every 32nd page of this warp's
-  int u = u_begin + warp, ahead = 0, id = 0;
+  int u = u_begin + warp, ahead = 0;
   auto ids = [&](int from) { id = from + lane * warps < u_end ? pages[page_of(from + lane * warps)] : 0; };
-  ids(u);
+  if (a.window > 0) ids(u);
   auto ask = [&](bool values, int64_t page, bool skip) {         // (lane 0)
     uint64_t* bar = &bars[values ? 1 : 0];
     const int64_t cell = (page * a.kv_heads + kvh) * PAGE;
@@ -458,7 +460,8 @@ attention_int8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     if (a.splits > 1) {
       float* dst = a.scratch + ((row * a.n_heads + h0 + head) * a.splits + split) * (a.hd + 2);
       if (d2 == 0) dst[a.hd] = top, dst[a.hd + 1] = l;
-      if (busy > 0) dst[d2 * 2] = x.x, dst[d2 * 2 + 1] = x.y;
+      dst[d2 * 2] = x.x;                          // (zeros where the block has no pages)
+      dst[d2 * 2 + 1] = x.y;
     } else {
       T* dst = reinterpret_cast<T*>(a.out) + row * a.ld_out + (int64_t)(h0 + head) * a.hd + d2 * 2;
       const float inv = 1.f / l;
@@ -468,33 +471,38 @@ attention_int8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   }
 }
 
-// The blocks of a row and head meet: a warp for each.
+// The blocks of a row and head meet: four warps for each, a quarter of the blocks a warp, a lane every 32nd entry.
 template <typename T>
 __global__ void __launch_bounds__(128)
-attention_int8_join_kernel(const float* __restrict__ scratch, T* __restrict__ out, int64_t ld_out, int n_rows, int n_heads, int hd, int splits) {
+attention_int8_join_kernel(const float* __restrict__ scratch, T* __restrict__ out, int64_t ld_out, int n_heads, int hd, int splits) {
+  __shared__ float parts[4][256 + 1];
   pdl_launch_dependents();
-  const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  pdl_wait();
-  if (item >= (int64_t)n_rows * n_heads) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t item = blockIdx.x;
   const float* src = scratch + item * splits * (hd + 2);
+  pdl_wait();
   float top = -INFINITY;
-  for (int s = 0; s < splits; ++s) top = fmaxf(top, src[s * (hd + 2) + hd]);
+  for (int s = lane; s < splits; s += 32) top = fmaxf(top, src[s * (hd + 2) + hd]);
+  top = warp_max(top);
   float x[8] = {}, l = 0.f;
-  for (int s = 0; s < splits; ++s) {
-    const float m = src[s * (hd + 2) + hd];
-    if (m == -INFINITY) continue;                                // (a block without pages leaves no output)
-    const float f = exp2_fast(m - top);
-    l = fmaf(src[s * (hd + 2) + hd + 1], f, l);
+#pragma unroll 4
+  for (int s = warp; s < splits; s += 4) {
+    const float* block = src + s * (hd + 2);
+    const float m = block[hd], f = m == -INFINITY ? 0.f : exp2_fast(m - top);
+    l = fmaf(block[hd + 1], f, l);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i * 32 + lane < hd) x[i] = fmaf(src[s * (hd + 2) + i * 32 + lane], f, x[i]);
+      if (i * 32 + lane < hd) x[i] = fmaf(block[i * 32 + lane], f, x[i]);
   }
-  const int64_t row = item / n_heads;
-  T* dst = out + row * ld_out + (item - row * n_heads) * hd;
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    if (i * 32 + lane < hd) dst[i * 32 + lane] = from_f32<T>(x[i] / l);
+    if (i * 32 + lane < hd) parts[warp][i * 32 + lane] = x[i];
+  if (lane == 0) parts[warp][256] = l;
+  __syncthreads();
+  const int64_t row = item / n_heads;
+  T* dst = out + row * ld_out + (item - row * n_heads) * hd;
+  const float inv = 1.f / ((parts[0][256] + parts[1][256]) + (parts[2][256] + parts[3][256]));
+  for (int i = threadIdx.x; i < hd; i += 128) dst[i] = from_f32<T>(((parts[0][i] + parts[1][i]) + (parts[2][i] + parts[3][i])) * inv);
 }
 
 // [rows of all pages][hd] bytes, a page's rows a copy.
@@ -547,10 +555,10 @@ int by_size(const Args& a, const int8_t* k, const int8_t* v, int64_t cache_rows,
   const int rc = a.hd <= 16 ? go(std::integral_constant<int, 16>()) : a.hd <= 32 ? go(std::integral_constant<int, 32>())
                  : a.hd <= 64 ? go(std::integral_constant<int, 64>()) : a.hd <= 128 ? go(std::integral_constant<int, 128>()) : go(std::integral_constant<int, 256>());
   if (rc != KVAD_OK || a.splits == 1) return rc;
-  const int64_t blocks = ((int64_t)n_rows * a.n_heads + 3) / 4;
+  const int64_t blocks = (int64_t)n_rows * a.n_heads;
   KVAD_REQUIRE(blocks < (1ll << 31), "attention_int8: more rows and heads than a launch takes");
   const cudaError_t e = kvad_launch(attention_int8_join_kernel<T>, dim3((unsigned)blocks), dim3(128), 0, stream, (const float*)a.scratch,
-                                    reinterpret_cast<T*>(a.out), a.ld_out, n_rows, a.n_heads, a.hd, a.splits);
+                                    reinterpret_cast<T*>(a.out), a.ld_out, a.n_heads, a.hd, a.splits);
   if (e != cudaSuccess) KVAD_FAIL(KVAD_ERR_CUDA, "attention_int8: launch failed: %s", cudaGetErrorString(e));
   return KVAD_OK;
 }

@@ -541,7 +541,13 @@ KVAD_EXPORT int kvad_attention_int8_prompt(const void* q, int64_t ld_q, void* ou
          n_seqs, n_heads, kv_heads, window, window > 0 ? keep_first : 0, g_skip_copy ? 1 : 0, scale * LOG2E};
   g_skip_copy = false;
   switch (hd) {
+    case 16: return launch<16>(q, ld_q, n_rows, a, max_new, stream);
+    case 32: return launch<32>(q, ld_q, n_rows, a, max_new, stream);
+    case 48: return launch<48>(q, ld_q, n_rows, a, max_new, stream);
     case 64: return launch<64>(q, ld_q, n_rows, a, max_new, stream);
+    case 80: return launch<80>(q, ld_q, n_rows, a, max_new, stream);
+    case 96: return launch<96>(q, ld_q, n_rows, a, max_new, stream);
+    case 112: return launch<112>(q, ld_q, n_rows, a, max_new, stream);
     case 128: return launch<128>(q, ld_q, n_rows, a, max_new, stream);
     default: KVAD_FAIL(KVAD_ERR_UNSUPPORTED, "attention_int8_prompt: no kernel for heads of %d entries", hd);
   }

@@ -1946,7 +1946,7 @@ class Ops:
                                    page_table.shape[1], k_pages.data_ptr(), k_scales.data_ptr(), v_pages.data_ptr(), v_scales.data_ptr(), n, n_kv, hd, page,
                                    _stream()), h)
 
-    INT8_PROMPT_HEAD_SIZES = (64, 128)
+    INT8_PROMPT_HEAD_SIZES = (16, 32, 48, 64, 80, 96, 112, 128)
 
     def attention_int8(self, q, out, seq_starts, kv_lens, n_seqs: int, max_new: int, page_table, k_pages, k_scales, v_pages, v_scales, n_heads: int,
                        scale: float, *, window: int = 0, keep_first: int = 0) -> None:
@@ -1991,13 +1991,17 @@ class Ops:
     @staticmethod
     def int8_splits(items: int, reach: int, n_sms: Optional[int] = None) -> tuple:
         """How single-token rows deal out the pages of a sequence and key/value head (`items` of them, `reach` pages each at most): (blocks, pages a block,
-        warps a block).  Up to 16 pages one block of eight warps has them all; beyond, blocks of four warps, two an SM at least where four pages (one a
-        warp) are left to each, and 16 pages a block at most, so that sequences of unequal lengths keep all SMs busy."""
-        if reach <= 16:
-            return 1, 0, 8
-        want = -(-2 * (n_sms or sm_count()) // max(1, items))
-        pages = max(4, min(16, -(-reach // want)))
-        return -(-reach // pages), pages, 4
+        warps a block).  Up to as many items as SMs: blocks of eight warps, one an SM, whole rounds of their warps; up to 16 pages one block has them all (it takes
+        a second launch to join several).  More items: blocks of four warps, three an SM, with 48 pages at most, so that sequences of unequal lengths
+        keep all SMs busy.  (us, heads of 128 in fours, one sequence of 8000 positions, 8 heads: 8, 16, 32 pages for eight warps 13.5, 13.5, 17.5, for four
+        14.3, 16.3, 21.8; of 30000: 36.8, 27.5, 21.6; 8 sequences of 4000: 32.1, 25.0, 20.4, all 26.5; 64 of 1000..8192: 32, 48 pages for four warps
+        115, 111, all for eight 115.  64 sequences of 520, 12 heads of 64: all for eight 23.2, for four 21.8; one of 520: 7.4, 8.2.)"""
+        sms = n_sms or sm_count()
+        if items > sms:
+            return -(-reach // 48), 48, 4
+        blocks = max(1, sms // max(1, items)) if reach > 16 else 1
+        pages = -(-reach // (8 * blocks)) * 8
+        return -(-reach // pages), pages, 8
 
     # -- sampling ------------------------------------------------------------------
     ARGMAX_CHUNK = 2048
