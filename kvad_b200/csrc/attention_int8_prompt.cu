@@ -68,7 +68,7 @@ template <int HD> struct Layout {
   static constexpr uint32_t SET = 16 + PAGE * 4;                 // what softmax threads need of a page, and marks of its keys
   static constexpr uint32_t OFF_KV = 2 * Q_BYTES, OFF_RAW = OFF_KV + RING * KV_BYTES, OFF_SC = OFF_RAW + RAW * RAW_BYTES;
   static constexpr uint32_t OFF_BAR = OFF_SC + SETS * SET;
-  static constexpr int BARS = 1 + 2 * RING + 2 * RAW + 2 * 6;
+  static constexpr int BARS = 1 + 2 * RING + 2 * RAW + 2 * 7;
   static constexpr size_t SMEM = OFF_BAR + BARS * 8 + 16 + 1024;
   static constexpr uint32_t TM_O = 256;                          // S (and P) of slot t at t * 128 + 64 in turn, its output at TM_O + t * 128
   static_assert(SETS >= RING / 2 + 2, "a page's set is read until the products of the page before are done");
@@ -129,6 +129,26 @@ __device__ __forceinline__ float power_of_2(int e) { return __uint_as_float((uin
 __host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool b_mn_major) {
   return (1u << 4) | (b_mn_major ? (1u << 16) : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
+// Sixteen columns of a row from tensor memory, there when the statement is over.  (One statement for the load and the wait: between two, the compiler is free to work on
+// registers that are still on their way.)
+__device__ __forceinline__ void tmem_read16(uint32_t addr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(addr) : "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+// Waits for a page's scores that have been asked for.  (The registers go through the statement, so that nothing that works on them comes before it.)
+__device__ __forceinline__ void tmem_arrived(uint32_t (&x)[PAGE]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(x[0]), "+r"(x[1]), "+r"(x[2]), "+r"(x[3]), "+r"(x[4]), "+r"(x[5]), "+r"(x[6]), "+r"(x[7]), "+r"(x[8]), "+r"(x[9]), "+r"(x[10]), "+r"(x[11]), "+r"(x[12]), "+r"(x[13]), "+r"(x[14]), "+r"(x[15]), "+r"(x[16]), "+r"(x[17]), "+r"(x[18]), "+r"(x[19]), "+r"(x[20]), "+r"(x[21]), "+r"(x[22]), "+r"(x[23]), "+r"(x[24]), "+r"(x[25]), "+r"(x[26]), "+r"(x[27]), "+r"(x[28]), "+r"(x[29]), "+r"(x[30]), "+r"(x[31])
+               : : "memory");
+  asm volatile(""
+               : "+r"(x[32]), "+r"(x[33]), "+r"(x[34]), "+r"(x[35]), "+r"(x[36]), "+r"(x[37]), "+r"(x[38]), "+r"(x[39]), "+r"(x[40]), "+r"(x[41]), "+r"(x[42]), "+r"(x[43]), "+r"(x[44]), "+r"(x[45]), "+r"(x[46]), "+r"(x[47]), "+r"(x[48]), "+r"(x[49]), "+r"(x[50]), "+r"(x[51]), "+r"(x[52]), "+r"(x[53]), "+r"(x[54]), "+r"(x[55]), "+r"(x[56]), "+r"(x[57]), "+r"(x[58]), "+r"(x[59]), "+r"(x[60]), "+r"(x[61]), "+r"(x[62]), "+r"(x[63])
+               : : "memory");
+}
+
 template <int HD>
 __global__ void __launch_bounds__(THREADS, 1)
 attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ Args a) {
@@ -147,8 +167,8 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
   uint64_t* raw_empty = raw_full + RAW;                          // [RAW] they have been turned
   uint64_t* s_full = raw_empty + RAW;                            // [slot][2] S is in tensor memory
   uint64_t* p_full = s_full + 4;                                 // [slot][2] P is (and S has been read)
-  uint64_t* t_full = p_full + 4;                                 // [slot] P V has been added
-  uint64_t* q_ready = t_full + 2;                                // [slot] its queries are half precision
+  uint64_t* t_full = p_full + 4;                                 // [slot][2] P V of a page has been added (two in turn: a wait for the latest must not take one before for it)
+  uint64_t* q_ready = t_full + 4;                                // [slot] its queries are half precision
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_ready + 2);
   __shared__ int failed;
 
@@ -178,8 +198,8 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
     mbar_init(q_full, 1);
     for (int i = 0; i < RING; ++i) { mbar_init(&kv_full[i], 128); mbar_init(&kv_empty[i], 2); }
     for (int i = 0; i < RAW; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 4); }
-    for (int i = 0; i < 4; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&t_full[i], 1); mbar_init(&q_ready[i], 128); }
+    for (int i = 0; i < 4; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); mbar_init(&t_full[i], 1); }
+    for (int i = 0; i < 2; ++i) mbar_init(&q_ready[i], 128);
     failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_shared();
@@ -231,7 +251,7 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
       // keys of page i + 1, then values of page i: from page -1 on, which has no values, to the last, which has no next
       for (int i = -1; i < units && ok; ++i) {
         if (i + 1 < units) {
-          if (i + 1 < mine && i > 0 && !mbar_wait(&t_full[t], (i - 1) & 1)) { ok = false; break; }      // P V of page i - 1 has read what S goes over
+          if (i + 1 < mine && i > 0 && !mbar_wait(&t_full[t * 2 + ((i - 1) & 1)], ((i - 1) >> 1) & 1)) { ok = false; break; }      // P V of page i - 1 has read what S goes over
           if (!mbar_wait(&kv_full[r], phase)) { ok = false; break; }
           if (i + 1 < mine) {
             tc_fence_after();
@@ -258,7 +278,7 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
               const uint64_t at = v_desc + (uint32_t)r * (L::KV_BYTES >> 4);
 #pragma unroll
               for (int k = 0; k < PAGE / 16; ++k) umma_ta(tm_o, tm_s + (i & 1) * PAGE + k * 8, at + (uint64_t)(k * (2048 >> 4)), idesc_t, (i > 0 || k > 0) ? 1u : 0u);
-              umma_commit(&t_full[t]);
+              umma_commit(&t_full[t * 2 + (i & 1)]);
               umma_commit(&kv_empty[r]);
             }
           } else if (lane == 0) {
@@ -397,7 +417,7 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
       tmem_ld32(tm_s + b * PAGE + 32, x + 32);
       const float4 about = *reinterpret_cast<const float4*>(set);
       const float mul = fmaxf(about.x * row_mul, 0x1p-126f);
-      tmem_ld_wait();
+      tmem_arrived(x);
       const int last = pos - page * PAGE;        // the last key of the page that the row sees
       if (page * PAGE + PAGE - 1 > first_pos) {
 #pragma unroll
@@ -420,7 +440,7 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
       if (i == 0) {
         ref = peak;
       } else if (__any_sync(0xffffffffu, peak > ref + RISE)) {
-        if (!mbar_wait(&t_full[t], (i - 1) & 1)) { ok = false; break; }      // the output is at rest
+        if (!mbar_wait(&t_full[t * 2 + ((i - 1) & 1)], ((i - 1) >> 1) & 1)) { ok = false; break; }      // the output is at rest
         tc_fence_after();
         const float to = fmaxf(ref, peak), keep = ref == -INFINITY ? 0.f : exp2_fast(ref - to);
         sum *= keep;
@@ -428,7 +448,7 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
 #pragma unroll
         for (int c0 = 0; c0 < HD; c0 += 16) {
           float o[16];
-          tmem_ld16(tm_o + c0, o);
+          tmem_read16(tm_o + c0, o);
           uint32_t w[2][8];
 #pragma unroll
           for (int c = 0; c < 16; ++c) w[c >> 3][c & 7] = __float_as_uint(o[c] * keep);
@@ -461,7 +481,7 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
       mbar_arrive_one(&p_full[t * 2 + b]);
     }
     if (ok && mine > 0) {
-      ok = mbar_wait(&t_full[t], (mine - 1) & 1);
+      ok = mbar_wait(&t_full[t * 2 + ((mine - 1) & 1)], ((mine - 1) >> 1) & 1);
       tc_fence_after();
       const float inv = 1.f / (sum * SHIFT);
       const int token = row / group, head = row - token * group;
@@ -470,7 +490,7 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
 #pragma unroll
       for (int c0 = 0; c0 < HD; c0 += 16) {
         float o[16];
-        tmem_ld16(tm_o + c0, o);
+        tmem_read16(tm_o + c0, o);
         if (there) {
           uint32_t w[8];
 #pragma unroll

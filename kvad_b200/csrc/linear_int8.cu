@@ -157,6 +157,17 @@ __device__ __forceinline__ void umma_i8(uint32_t d, uint64_t a_desc, uint64_t b_
       ::"r"(d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(zero) : "memory");
 }
 
+// Sixteen columns of a row from tensor memory, there when the statement is over.  (One statement for the load and the wait: between two, the compiler is free to work on
+// registers that are still on their way.)
+__device__ __forceinline__ void tmem_read16(uint32_t addr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(addr) : "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
 // Sixteen consecutive entries of a vector from `n` on, zeros beyond N.
 __device__ __forceinline__ void load16(const float* p, int n, int N, float* v) {
   if (n + 16 <= N && (reinterpret_cast<uintptr_t>(p + n) & 15) == 0) {
@@ -304,7 +315,7 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
         for (int cc = 0; cc < SLAB; cc += 16) {
           float v[16], s[16];
           load16(o.sw, n0 + c0 + cc, N, s);
-          tmem_ld16(acc + (uint32_t)(c0 + cc), v);
+          tmem_read16(acc + (uint32_t)(c0 + cc), v);
 #pragma unroll
           for (int j = 0; j < 16; ++j) v[j] = (float)__float_as_int(v[j]) * sa * s[j];
           if (o.bias != nullptr) {
