@@ -1,7 +1,8 @@
 """Device storage of the cache.
 
 For every key/value group: two tensors `[layers of the group, pages,
-kv heads, 64, head size]` in the engine's dtype.  A page of one head is one
+kv heads, 64, head size]` in the engine's dtype, or as 8-bit codes with two
+tensors of scales `[layers of the group, pages, kv heads, 64]` beside them.  A page of one head is one
 contiguous tile, which is what the attention kernels read.  For every state
 group: `[layers of the group, slots, *shape]`, zeroed when a slot is handed
 out (bisand/kvad zeroes `CacheShape.state` the same way,
@@ -34,6 +35,8 @@ class KVView:
     page_size: int
     keep_first: int = 0
     chunk: Optional[int] = None
+    k_scales: Optional[torch.Tensor] = None    # float32 [pages, kv heads, page size] of a group in 8 bits
+    v_scales: Optional[torch.Tensor] = None
 
 
 class DeviceCache:
@@ -53,6 +56,7 @@ class DeviceCache:
         self.table_width = max(1, -(-per_seq // page_size))
 
         self.kv: dict[int, tuple[torch.Tensor, Optional[torch.Tensor]]] = {}
+        self.scales: dict[int, tuple[torch.Tensor, torch.Tensor]] = {}     # of groups in 8 bits: keys', values'
         self.state: dict[int, torch.Tensor] = {}
         pages_per_group, windows, keep_first, chunks = [], [], [], []
         self._kv_group_index: dict[int, int] = {}     # layout group -> index among kv groups (SlotBook's numbering)
@@ -60,9 +64,12 @@ class DeviceCache:
             need = group.need
             if isinstance(need, KVNeed):
                 shape = (len(group.entries), n_pages, need.n_kv_heads, page_size)
-                self.kv[g] = (torch.empty((*shape, need.head_dim), dtype=dtype, device=self.device),
-                              torch.empty((len(group.entries), n_pages, need.v_heads, page_size, need.v_dim), dtype=dtype, device=self.device)
+                held = torch.int8 if need.int8 else dtype
+                self.kv[g] = (torch.empty((*shape, need.head_dim), dtype=held, device=self.device),
+                              torch.empty((len(group.entries), n_pages, need.v_heads, page_size, need.v_dim), dtype=held, device=self.device)
                               if need.v_dim else None)
+                if need.int8:
+                    self.scales[g] = tuple(torch.empty(shape, dtype=torch.float32, device=self.device) for _ in range(2))
                 self._kv_group_index[g] = len(pages_per_group)
                 pages_per_group.append(n_pages)
                 windows.append(need.window)
@@ -97,7 +104,9 @@ class DeviceCache:
         g, i = self.layout.place(entry)
         k, v = self.kv[g]
         need = self.layout.groups[g].need
-        return KVView(k[i], None if v is None else v[i], page_tables[g], need.window, self.page_size, need.keep_first, need.chunk)
+        ks, vs = self.scales.get(g, (None, None))
+        return KVView(k[i], None if v is None else v[i], page_tables[g], need.window, self.page_size, need.keep_first, need.chunk,
+                      None if ks is None else ks[i], None if vs is None else vs[i])
 
     def state_view(self, entry: int) -> torch.Tensor:
         """`[slots, *shape]` of one entry; rows are indexed by slot id."""
@@ -109,6 +118,8 @@ class DeviceCache:
         n = 0
         for k, v in self.kv.values():
             n += k.numel() * k.element_size() + (0 if v is None else v.numel() * v.element_size())
+        for ks, vs in self.scales.values():
+            n += (ks.numel() + vs.numel()) * 4
         for s in self.state.values():
             n += s.numel() * s.element_size()
         return n

@@ -24,6 +24,7 @@ class KVNeed:
     keep_first: int = 0              # with a window: the first positions stay in reach of every later query
     chunk: Optional[int] = None      # queries reach back to the start of their own chunk of so many positions, counted from position 0
     value_heads: Optional[int] = None  # None: as many value heads as key heads; else fewer (several key heads read one value head)
+    int8: bool = False               # keys and values are held as 8-bit codes with a 32-bit scale for each position and head
 
     def __post_init__(self):
         if self.n_kv_heads <= 0 or self.head_dim <= 0:
@@ -36,6 +37,8 @@ class KVNeed:
             raise ValueError("value size and kept first positions cannot be negative")
         if self.value_heads is not None and (self.value_heads <= 0 or self.n_kv_heads % self.value_heads):
             raise ValueError("the key heads must divide evenly over the value heads")
+        if self.int8 and (self.v_dim != self.head_dim or self.v_heads != self.n_kv_heads):
+            raise ValueError("a cache in 8 bits holds values like its keys")
 
     @property
     def v_dim(self) -> int:
@@ -98,5 +101,8 @@ class CacheLayout:
         total = 0
         for g in self.groups:
             if isinstance(g.need, KVNeed):
-                total += len(g.entries) * (g.need.n_kv_heads * g.need.head_dim + g.need.v_heads * g.need.v_dim) * element_size
+                if g.need.int8:
+                    total += len(g.entries) * 2 * g.need.n_kv_heads * (g.need.head_dim + 4)
+                else:
+                    total += len(g.entries) * (g.need.n_kv_heads * g.need.head_dim + g.need.v_heads * g.need.v_dim) * element_size
         return total

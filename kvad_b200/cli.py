@@ -44,6 +44,7 @@ def build_parser() -> argparse.ArgumentParser:
     run.add_argument("--seed", type=int, default=7, help="same seed, same text")
     run.add_argument("--greedy", action="store_true", help="--temperature 0")
     run.add_argument("--dtype", default="bf16", choices=["bf16", "bfloat16", "f32", "float32"])
+    run.add_argument("--int8", action="store_true", help="the blocks' products and the cache in 8 bits (GPT-2)")
     run.add_argument("--stop", type=int, action="append", help="a stop token id (default: the model's eos ids)")
     run.add_argument("--random-weights", metavar="CONFIG", help="write random weights for CONFIG (a config.json) into --model first")
     run.add_argument("--cache-tokens", type=int, default=0, help="size of the cache in tokens (default: what the prompts need)")
@@ -109,7 +110,7 @@ def cmd_run(args) -> int:
     temperature = 0.0 if args.greedy else args.temperature
     t0 = time.time()
     need = sum(-(-(len(p) + args.max_tokens) // 64) * 64 for p in prompts)
-    engine = Engine.from_pretrained(args.model, args.dtype, max_tokens=max(args.cache_tokens, need))
+    engine = Engine.from_pretrained(args.model, args.dtype, max_tokens=max(args.cache_tokens, need), int8=args.int8)
     _say(engine.describe())
     _say(f"loaded in {time.time() - t0:.1f} s")
     outs, stats = engine.generate(prompts, max_tokens=args.max_tokens, temperature=temperature, top_k=args.top_k,

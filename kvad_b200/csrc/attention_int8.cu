@@ -25,7 +25,7 @@
 #include <type_traits>
 
 #include "common.cuh"
-#include "tcgen05.cuh"
+#include "attention_int8_join.cuh"
 
 using namespace kvad;
 
@@ -48,7 +48,8 @@ struct Args {
   const int* table;
   const float* ks;
   const float* vs;
-  float* scratch;                               // [rows][heads][splits][hd + 2] where a row's pages are dealt out to several blocks
+  float* scratch;                               // where a row's pages are dealt out to several blocks: see attention_int8_join.cuh
+  int64_t items;                                // rows x heads
   int table_width, n_seqs, n_heads, kv_heads, hd, window, keep_first, splits, split_pages, skip_copy;
   float scale_log2;
 };
@@ -67,11 +68,6 @@ template <int HDP, int PIECES, int NT> struct Layout {
 
 __device__ __forceinline__ uint32_t as_bits(__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); }
 __device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ float power_of_2(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
 __device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
@@ -334,7 +330,7 @@ attention_int8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         for (int x = 4; x < 32; x *= 2) top_score = fmaxf(top_score, __shfl_xor_sync(0xffffffffu, top_score, x));
         const float to = fmaxf(ref[n][e], top_score + c);
         changed |= to != ref[n][e];
-        keep[n][e] = to == -INFINITY ? 1.f : exp2_fast(ref[n][e] - to);
+        keep[n][e] = to == -INFINITY ? 1.f : exp2_near(ref[n][e] - to);
         ref[n][e] = to;
         const float add = c + HEAD - (to == -INFINITY ? 0.f : to);
         float part = 0.f;
@@ -342,7 +338,7 @@ attention_int8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         for (int m = 0; m < 4; ++m)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float p = exp2_fast(sc[m][n][e + 2 * h] + add);
+            const float p = exp2_near(sc[m][n][e + 2 * h] + add);
             part += p;
             const float w = p * v_by[m][h];
             sc[m][n][e + 2 * h] = masked && sc[m][n][e + 2 * h] == -INFINITY ? 0.f : w;      // (a scale that is not finite is for those alone who see it)
@@ -450,7 +446,7 @@ attention_int8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     for (int w = 0; w < busy; ++w) top = fmaxf(top, reinterpret_cast<const float*>(base + w * stride + 2 * L::TILE)[r]);
     for (int w = 0; w < busy; ++w) {
       const float* m = reinterpret_cast<const float*>(base + w * stride + 2 * L::TILE);
-      const float f = m[r] == -INFINITY ? 0.f : exp2_fast(m[r] - top);
+      const float f = m[r] == -INFINITY ? 0.f : exp2_near(m[r] - top);
       const float2 y = reinterpret_cast<const float2*>(base + w * stride)[r * (HDP / 2) + (d2 ^ (((r & 6) * 4) & TURN))];
       l = fmaf(m[PAGE + r], f, l);
       x.x = fmaf(y.x, f, x.x);
@@ -458,10 +454,9 @@ attention_int8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     }
     const int64_t row = row0 + tile * tok + token;
     if (a.splits > 1) {
-      float* dst = a.scratch + ((row * a.n_heads + h0 + head) * a.splits + split) * (a.hd + 2);
-      if (d2 == 0) dst[a.hd] = top, dst[a.hd + 1] = l;
-      dst[d2 * 2] = x.x;                          // (zeros where the block has no pages)
-      dst[d2 * 2 + 1] = x.y;
+      const int64_t place = (row * a.n_heads + h0 + head) * a.splits + split;
+      if (d2 == 0) reinterpret_cast<float2*>(a.scratch + a.items * a.splits * a.hd)[place] = make_float2(top, l);
+      if (busy > 0) reinterpret_cast<float2*>(a.scratch + place * a.hd)[d2] = x;
     } else {
       T* dst = reinterpret_cast<T*>(a.out) + row * a.ld_out + (int64_t)(h0 + head) * a.hd + d2 * 2;
       const float inv = 1.f / l;
@@ -469,40 +464,6 @@ attention_int8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
       dst[1] = from_f32<T>(x.y * inv);
     }
   }
-}
-
-// The blocks of a row and head meet: four warps for each, a quarter of the blocks a warp, a lane every 32nd entry.
-template <typename T>
-__global__ void __launch_bounds__(128)
-attention_int8_join_kernel(const float* __restrict__ scratch, T* __restrict__ out, int64_t ld_out, int n_heads, int hd, int splits) {
-  __shared__ float parts[4][256 + 1];
-  pdl_launch_dependents();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t item = blockIdx.x;
-  const float* src = scratch + item * splits * (hd + 2);
-  pdl_wait();
-  float top = -INFINITY;
-  for (int s = lane; s < splits; s += 32) top = fmaxf(top, src[s * (hd + 2) + hd]);
-  top = warp_max(top);
-  float x[8] = {}, l = 0.f;
-#pragma unroll 4
-  for (int s = warp; s < splits; s += 4) {
-    const float* block = src + s * (hd + 2);
-    const float m = block[hd], f = m == -INFINITY ? 0.f : exp2_fast(m - top);
-    l = fmaf(block[hd + 1], f, l);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i * 32 + lane < hd) x[i] = fmaf(block[i * 32 + lane], f, x[i]);
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i * 32 + lane < hd) parts[warp][i * 32 + lane] = x[i];
-  if (lane == 0) parts[warp][256] = l;
-  __syncthreads();
-  const int64_t row = item / n_heads;
-  T* dst = out + row * ld_out + (item - row * n_heads) * hd;
-  const float inv = 1.f / ((parts[0][256] + parts[1][256]) + (parts[2][256] + parts[3][256]));
-  for (int i = threadIdx.x; i < hd; i += 128) dst[i] = from_f32<T>(((parts[0][i] + parts[1][i]) + (parts[2][i] + parts[3][i])) * inv);
 }
 
 // [rows of all pages][hd] bytes, a page's rows a copy.
@@ -555,10 +516,7 @@ int by_size(const Args& a, const int8_t* k, const int8_t* v, int64_t cache_rows,
   const int rc = a.hd <= 16 ? go(std::integral_constant<int, 16>()) : a.hd <= 32 ? go(std::integral_constant<int, 32>())
                  : a.hd <= 64 ? go(std::integral_constant<int, 64>()) : a.hd <= 128 ? go(std::integral_constant<int, 128>()) : go(std::integral_constant<int, 256>());
   if (rc != KVAD_OK || a.splits == 1) return rc;
-  const int64_t blocks = (int64_t)n_rows * a.n_heads;
-  KVAD_REQUIRE(blocks < (1ll << 31), "attention_int8: more rows and heads than a launch takes");
-  const cudaError_t e = kvad_launch(attention_int8_join_kernel<T>, dim3((unsigned)blocks), dim3(128), 0, stream, (const float*)a.scratch,
-                                    reinterpret_cast<T*>(a.out), a.ld_out, a.n_heads, a.hd, a.splits);
+  const cudaError_t e = join_blocks<T>(a.scratch, a.out, a.ld_out, n_rows, a.n_heads, a.hd, a.splits, stream);
   if (e != cudaSuccess) KVAD_FAIL(KVAD_ERR_CUDA, "attention_int8: launch failed: %s", cudaGetErrorString(e));
   return KVAD_OK;
 }
@@ -582,7 +540,7 @@ KVAD_EXPORT int kvad_attention_int8(int dtype, const void* q, int64_t ld_q, void
                splits, split_pages, warps);
   const int64_t cache_rows = (int64_t)n_pages * kv_heads * PAGE;
   KVAD_REQUIRE(cache_rows < (1ll << 31), "attention_int8: more cached rows than a copy can name");
-  const Args a{q, ld_q, out, ld_o, seq_starts, kv_lens, table, k_scales, v_scales, reinterpret_cast<float*>(scratch), table_width, n_seqs, n_heads, kv_heads, hd,
+  const Args a{q, ld_q, out, ld_o, seq_starts, kv_lens, table, k_scales, v_scales, reinterpret_cast<float*>(scratch), (int64_t)n_rows * n_heads, table_width, n_seqs, n_heads, kv_heads, hd,
                window, window > 0 ? keep_first : 0, splits, split_pages, g_skip_copy ? 1 : 0, scale * LOG2E};
   g_skip_copy = false;
   const int rc = dtype == KVAD_DTYPE_F32 ? by_size<float>(a, k_pages, v_pages, cache_rows, n_rows, max_new, warps, stream)

@@ -1,0 +1,82 @@
+// What several blocks that share a row of attention over 8-bit caches leave, and the kernel that joins it.  With item = row x heads + head and place = item x blocks + block:
+//
+//   scratch[place hd ..]                          the output relative to 2^m, not yet divided by the sum
+//   scratch[items blocks hd + 2 place ..]         m, the power of two, and the sum relative to it
+//
+// m is minus infinity where the block had no pages for the row; nothing else is left then.
+#pragma once
+#include "tcgen05.cuh"
+
+namespace kvad {
+
+__device__ __forceinline__ float exp2_near(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The blocks of a row and head meet.  W warps for each, which share the blocks out among them, 4 / W items a block of threads; a lane has every 32nd entry.
+template <typename T, int W>
+__global__ void __launch_bounds__(128)
+attention_int8_join_kernel(const float* scratch, T* out, int64_t ld_out, int64_t items, int n_heads, int hd, int splits) {
+  __shared__ float parts[W == 1 ? 1 : W][256 + 1];
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % W;
+  const int64_t item = (int64_t)blockIdx.x * (4 / W) + (threadIdx.x >> 5) / W;
+  pdl_wait();
+  if (item >= items) return;                      // (only where an item is a warp's: no barrier follows)
+  const float* src = scratch + item * splits * hd;
+  const float2* about = reinterpret_cast<const float2*>(scratch + items * splits * hd) + item * splits;
+  float top = -INFINITY;
+  for (int s = lane; s < splits; s += 32) top = fmaxf(top, about[s].x);
+  top = warp_max(top);
+  float x[8] = {}, l = 0.f;
+#pragma unroll 4
+  for (int s = warp; s < splits; s += W) {
+    const float2 a = about[s];
+    const bool there = a.x != -INFINITY;
+    const float f = there ? exp2_near(a.x - top) : 0.f;
+    l = fmaf(there ? a.y : 0.f, f, l);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i * 32 + lane < hd) x[i] = fmaf(there ? src[(int64_t)s * hd + i * 32 + lane] : 0.f, f, x[i]);
+  }
+  const int64_t row = item / n_heads;
+  T* dst = out + row * ld_out + (item - row * n_heads) * hd;
+  if (W == 1) {
+    const float inv = 1.f / l;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i * 32 + lane < hd) dst[i * 32 + lane] = from_f32<T>(x[i] * inv);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i * 32 + lane < hd) parts[warp][i * 32 + lane] = x[i];
+  if (lane == 0) parts[warp][256] = l;
+  __syncthreads();
+  float sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < W; ++w) sum += parts[w][256];
+  const float inv = 1.f / sum;
+  for (int i = threadIdx.x; i < hd; i += 128) {
+    float y = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) y += parts[w][i];
+    dst[i] = from_f32<T>(y * inv);
+  }
+}
+
+// 0, or an error of the launch.
+template <typename T>
+static cudaError_t join_blocks(const float* scratch, void* out, int64_t ld_out, int n_rows, int n_heads, int hd, int splits, cudaStream_t stream) {
+  const int64_t items = (int64_t)n_rows * n_heads;
+  if (items >= (1ll << 31)) return cudaErrorInvalidConfiguration;
+  auto go = [&](auto kernel, int64_t blocks) {
+    return kvad_launch(kernel, dim3((unsigned)blocks), dim3(128), 0, stream, scratch, reinterpret_cast<T*>(out), ld_out, items, n_heads, hd, splits);
+  };
+  // (few items: four warps each, whatever there is to join: 32 of 8 blocks took 9 us by a warp each)
+  return splits > 8 || items <= 4096 ? go(attention_int8_join_kernel<T, 4>, items) : go(attention_int8_join_kernel<T, 1>, (items + 3) / 4);
+}
+
+}  // namespace kvad

@@ -28,6 +28,7 @@
 // Every wait is bounded; one that runs out raises a counter and the block frees its tensor memory and returns without writing.
 #include <cuda_fp16.h>
 
+#include "attention_int8_join.cuh"
 #include "scored_tiles.cuh"
 
 using namespace kvad;
@@ -56,8 +57,10 @@ struct Args {
   const float* ks;
   const int8_t* v;
   const float* vs;
-  int n_seqs, n_heads, kv_heads, window, keep_first, skip_copy;
+  int n_seqs, n_heads, kv_heads, window, keep_first, parts, part_pages, skip_copy;
   float scale_log2;
+  int64_t items;                                // rows x heads
+  float* scratch;                               // where the pages of a block's rows are dealt out to several blocks: see attention_int8_join.cuh
 };
 
 template <int HD> struct Layout {
@@ -94,11 +97,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
-}
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
   uint32_t r;
@@ -188,10 +186,19 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
   const int n_tok0 = min(tok, n_new - tok0), n_tok1 = max(0, min(tok, n_new - tok0 - tok));
   const int first_page = a.window > 0 ? max(0, pos0 - a.window + 1) / PAGE : 0;
   const int kept = min((a.keep_first + PAGE - 1) / PAGE, first_page);
-  const int units0 = kept + (pos0 + n_tok0 - 1) / PAGE - first_page + 1;
-  const int units1 = n_tok1 > 0 ? kept + (pos0 + tok + n_tok1 - 1) / PAGE - first_page + 1 : 0;
-  const int units = max(units0, units1);
-  auto page_of = [&](int u) { return u < kept ? u : first_page + u - kept; };
+  const int all0 = kept + (pos0 + n_tok0 - 1) / PAGE - first_page + 1;
+  const int all1 = n_tok1 > 0 ? kept + (pos0 + tok + n_tok1 - 1) / PAGE - first_page + 1 : 0;
+  // this block's share of them
+  const int part = blockIdx.y, first_unit = part * a.part_pages, most = a.parts > 1 ? a.part_pages : max(all0, all1);
+  const int units0 = min(max(all0 - first_unit, 0), most), units1 = min(max(all1 - first_unit, 0), most), units = max(units0, units1);
+  auto page_of = [&](int u) { return first_unit + u < kept ? first_unit + u : first_page + first_unit + u - kept; };
+  // a row's place in the scratch, and what is left beside it
+  auto place = [&](int t, int token, int head) { return ((int64_t)(row0 + tok0 + t * tok + token) * a.n_heads + kvh * group + head) * a.parts + part; };
+  auto leave = [&](int64_t at, float m, float sum) { reinterpret_cast<float2*>(a.scratch + a.items * a.parts * HD)[at] = make_float2(m, sum); };
+  if (units == 0) {
+    for (int r = threadIdx.x; r < (n_tok0 + n_tok1) * group; r += THREADS) leave(place(0, r / group, r % group), -INFINITY, 0.f);
+    return;
+  }
 
   if (threadIdx.x == 0) {
     prefetch_tensormap(&map_q);
@@ -442,7 +449,7 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
       } else if (__any_sync(0xffffffffu, peak > ref + RISE)) {
         if (!mbar_wait(&t_full[t * 2 + ((i - 1) & 1)], ((i - 1) >> 1) & 1)) { ok = false; break; }      // the output is at rest
         tc_fence_after();
-        const float to = fmaxf(ref, peak), keep = ref == -INFINITY ? 0.f : exp2_fast(ref - to);
+        const float to = fmaxf(ref, peak), keep = ref == -INFINITY ? 0.f : exp2_near(ref - to);
         sum *= keep;
         ref = to;
 #pragma unroll
@@ -466,8 +473,8 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
         for (int c = 0; c < 8; ++c) {
           float p, q;
           halves(fma2(pair(__uint_as_float(x[c0 + 2 * c]), __uint_as_float(x[c0 + 2 * c + 1])), mul2, add), p, q);
-          p = exp2_fast(p);
-          q = exp2_fast(q);
+          p = exp2_near(p);
+          q = exp2_near(q);
           part[c & 1] = add2(part[c & 1], pair(p, q));
           w[c] = f16_pair(p, q);
         }
@@ -480,18 +487,22 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
       tc_fence_before();
       mbar_arrive_one(&p_full[t * 2 + b]);
     }
+    const int token = row / group, head = row - token * group;
     if (ok && mine > 0) {
       ok = mbar_wait(&t_full[t * 2 + ((mine - 1) & 1)], ((mine - 1) >> 1) & 1);
       tc_fence_after();
-      const float inv = 1.f / (sum * SHIFT);
-      const int token = row / group, head = row - token * group;
       const bool there = ok && token < n_tok && !failed;
+      const float inv = 1.f / (a.parts > 1 ? SHIFT : sum * SHIFT);
       __nv_bfloat16* dst = a.out + (int64_t)(row0 + tok0 + t * tok + token) * a.ld_out + (int64_t)(kvh * group + head) * HD;
+      float* rest = a.parts > 1 && there ? a.scratch + place(t, token, head) * HD : nullptr;
 #pragma unroll
       for (int c0 = 0; c0 < HD; c0 += 16) {
         float o[16];
         tmem_read16(tm_o + c0, o);
-        if (there) {
+        if (rest != nullptr) {
+#pragma unroll
+          for (int c = 0; c < 16; c += 4) *reinterpret_cast<float4*>(rest + c0 + c) = make_float4(o[c] * inv, o[c + 1] * inv, o[c + 2] * inv, o[c + 3] * inv);
+        } else if (there) {
           uint32_t w[8];
 #pragma unroll
           for (int c = 0; c < 8; ++c) w[c] = bf16_pair(o[2 * c] * inv, o[2 * c + 1] * inv);
@@ -499,6 +510,9 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
           *reinterpret_cast<uint4*>(dst + c0 + 8) = make_uint4(w[4], w[5], w[6], w[7]);
         }
       }
+      if (rest != nullptr) leave(place(t, token, head), ref, sum);
+    } else if (a.parts > 1 && ok && token < n_tok) {
+      leave(place(t, token, head), -INFINITY, 0.f);
     }
   }
   if (!ok) failed = 1;
@@ -536,8 +550,9 @@ int launch(const void* q, int64_t ld_q, int n_rows, const Args& a, int max_new, 
     configured = true;
   }
   const int64_t blocks = (int64_t)((max_new + 2 * tok - 1) / (2 * tok)) * a.n_seqs * a.kv_heads;
-  KVAD_REQUIRE(blocks < (1ll << 31), "attention_int8_prompt: more rows and heads than a launch takes");
-  const cudaError_t e = kvad_launch(kernel, dim3((unsigned)blocks), dim3(THREADS), L::SMEM, stream, map, a);
+  KVAD_REQUIRE(blocks < (1ll << 31) && a.parts <= 65535, "attention_int8_prompt: more rows and heads than a launch takes");
+  cudaError_t e = kvad_launch(kernel, dim3((unsigned)blocks, a.parts), dim3(THREADS), L::SMEM, stream, map, a);
+  if (e == cudaSuccess && a.parts > 1) e = join_blocks<__nv_bfloat16>(a.scratch, a.out, a.ld_out, n_rows, a.n_heads, HD, a.parts, stream);
   if (e != cudaSuccess) KVAD_FAIL(KVAD_ERR_CUDA, "attention_int8_prompt: launch failed: %s", cudaGetErrorString(e));
   KVAD_CHECK_LAUNCH("attention_int8_prompt");
   return KVAD_OK;
@@ -545,10 +560,11 @@ int launch(const void* q, int64_t ld_q, int n_rows, const Args& a, int max_new, 
 
 }  // namespace
 
+// `parts` > 1: the pages that a block's rows see are dealt out to that many blocks, `part_pages` each, through `scratch` (float32, rows x heads x parts x (head size + 2)).
 KVAD_EXPORT int kvad_attention_int8_prompt(const void* q, int64_t ld_q, void* out, int64_t ld_o, const int* seq_starts, const int* kv_lens, const int* table,
                                            int table_width, const int8_t* k_pages, const float* k_scales, const int8_t* v_pages, const float* v_scales, int n_rows,
                                            int n_seqs, int max_new, int n_heads, int kv_heads, int hd, int page, float scale, int window, int keep_first,
-                                           cudaStream_t stream) {
+                                           int parts, int part_pages, void* scratch, cudaStream_t stream) {
   KVAD_REQUIRE(n_rows > 0 && n_seqs > 0 && max_new > 0 && table_width > 0, "attention_int8_prompt: needs rows, sequences and pages");
   KVAD_REQUIRE(n_heads > 0 && kv_heads > 0 && n_heads % kv_heads == 0, "attention_int8_prompt: %d heads do not divide into %d key/value heads", n_heads, kv_heads);
   KVAD_REQUIRE(page == PAGE, "attention_int8_prompt: pages hold 64 positions, not %d", page);
@@ -557,8 +573,9 @@ KVAD_EXPORT int kvad_attention_int8_prompt(const void* q, int64_t ld_q, void* ou
                  reinterpret_cast<uintptr_t>(k_scales) | reinterpret_cast<uintptr_t>(v_scales)) & 15) == 0 && ld_q % 8 == 0 && ld_o % 8 == 0,
                "attention_int8_prompt: rows, pages and scales must start on 16-byte boundaries");
   KVAD_REQUIRE(window >= 0 && keep_first >= 0, "attention_int8_prompt: a window and kept first positions cannot be negative");
+  KVAD_REQUIRE(parts >= 1 && (parts == 1 || (part_pages > 0 && scratch != nullptr)), "attention_int8_prompt: no way to deal out pages: %d, %d", parts, part_pages);
   Args a{reinterpret_cast<__nv_bfloat16*>(out), ld_o, seq_starts, kv_lens, table, table_width, k_pages, k_scales, v_pages, v_scales,
-         n_seqs, n_heads, kv_heads, window, window > 0 ? keep_first : 0, g_skip_copy ? 1 : 0, scale * LOG2E};
+         n_seqs, n_heads, kv_heads, window, window > 0 ? keep_first : 0, parts, part_pages, g_skip_copy ? 1 : 0, scale * LOG2E, (int64_t)n_rows * n_heads, reinterpret_cast<float*>(scratch)};
   g_skip_copy = false;
   switch (hd) {
     case 16: return launch<16>(q, ld_q, n_rows, a, max_new, stream);

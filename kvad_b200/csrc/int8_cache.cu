@@ -8,10 +8,13 @@
 // so a position takes head size + 4 bytes a head, where bfloat16 takes 2 * head size.
 //
 // A group of lanes (a power of two, head size / 8 at least) has one row: a lane brings eight entries, the group's maximum is a few shuffles, and
-// the codes leave as eight bytes a lane.  Keys and values go in one launch.  Bound by memory: 2 * (entry + 1) bytes a code, counting both directions.
+// the codes leave as eight bytes a lane.  A block has one head's keys or values of so many rows, four of them a group where there are many, all asked for before the
+// first is worked on.  Bound by memory: 2 * (entry + 1) bytes a code, counting both directions.
+//
+// No pointer is __restrict__: what is promised not to change may be read before the wait for the kernel that writes it.
 #include <type_traits>
 
-#include "common.cuh"
+#include "int8_codes.cuh"
 
 using namespace kvad;
 
@@ -67,76 +70,85 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, bool vec, const float* 
   }
 }
 
-// Which row of the cache a group of lanes has: (token row, head, keys or values).  -1: none.
-struct Place {
-  int64_t row;       // of the token, in the packed rows
-  int64_t cell;      // of the cache: (page * heads + head) * page size + place in the page
-  int head;
-  bool value;
-};
-__device__ __forceinline__ Place place_of(int64_t item, int heads, int page, const int* row_seq, const int* row_pos, const int* table, int table_width) {
-  Place p;
-  const int64_t rh = item >> 1;
-  p.value = item & 1;
-  p.row = rh / heads;
-  p.head = (int)(rh - p.row * heads);
-  const int pos = row_pos[p.row], pg = pos / page;
-  const int id = table[(int64_t)row_seq[p.row] * table_width + pg];
-  p.cell = ((int64_t)id * heads + p.head) * page + (pos - pg * page);
-  return p;
-}
-
-template <typename T, int LANES>
-__global__ void __launch_bounds__(256)
-int8_store_kernel(const T* __restrict__ k_src, const T* __restrict__ v_src, int64_t ld_src, int vec, const int* __restrict__ row_seq,
-                  const int* __restrict__ row_pos, const int* __restrict__ table, int table_width, int8_t* __restrict__ k_pages,
-                  float* __restrict__ k_scales, int8_t* __restrict__ v_pages, float* __restrict__ v_scales, int n, int heads, int hd, int page) {
-  pdl_launch_dependents();
-  const int lane = threadIdx.x % LANES;
-  const int64_t item = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
-  pdl_wait();
-  const bool has = item < (int64_t)n * heads * 2;
-  const bool in = has && lane * 8 < hd;
-  Place p{};
-  float v[8] = {};
-  if (has) p = place_of(item, heads, page, row_seq, row_pos, table, table_width);
-  if (in) load8((p.value ? v_src : k_src) + p.row * ld_src + (int64_t)p.head * hd + lane * 8, vec, v);
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-#pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (!in) return;
-  const bool finite = top < 0x7f800000u;
-  const float scale = finite ? __fmul_rn(__uint_as_float(top), 1.f / 127.f) : __uint_as_float(0x7fffffffu);
-  const bool some = finite && scale > 0.f;
-  uint32_t w[2] = {};
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float q = some ? __fdiv_rn(v[i], scale) : 0.f;
-    w[i >> 2] |= (uint32_t)(__float2int_rn(fminf(fmaxf(q, -127.f), 127.f)) & 0xff) << (8 * (i & 3));
+struct Pages {
+  const int* row_seq;
+  const int* row_pos;
+  const int* table;
+  int width, heads, hd, page, shift;      // shift: log2 of the page size; negative: it is no power of two
+  // Where the cache has row `row` and head `head`: (page * heads + head) * page size + place in the page.
+  __device__ __forceinline__ int64_t cell(int row, int head) const {
+    const int pos = row_pos[row], pg = shift >= 0 ? pos >> shift : pos / page;
+    return ((int64_t)table[(int64_t)row_seq[row] * width + pg] * heads + head) * page + (pos - pg * page);
   }
-  *reinterpret_cast<uint2*>((p.value ? v_pages : k_pages) + p.cell * hd + lane * 8) = make_uint2(w[0], w[1]);
-  if (lane == 0) (p.value ? v_scales : k_scales)[p.cell] = scale;
+};
+
+template <typename T, int LANES, int R>
+__global__ void __launch_bounds__(256)
+int8_store_kernel(const T* k_src, const T* v_src, int64_t ld_src, int vec, const Pages p, int8_t* k_pages,
+                  float* k_scales, int8_t* v_pages, float* v_scales, int n) {
+  constexpr int GROUPS = 256 / LANES;
+  pdl_launch_dependents();
+  const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES, head = blockIdx.y >> 1;
+  const bool value = blockIdx.y & 1, in = lane * 8 < p.hd;
+  const T* src = (value ? v_src : k_src) + (int64_t)head * p.hd + lane * 8;
+  const int row0 = blockIdx.x * (GROUPS * R) + group;
+  pdl_wait();
+  float v[R][8] = {};
+  int64_t cell[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int row = row0 + i * GROUPS;
+    if (row < n) {
+      if (in) load8(src + row * ld_src, vec, v[i]);
+      cell[i] = p.cell(row, head);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[i][e]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (!in || row0 + i * GROUPS >= n) continue;
+    const Scale k = scale_of(top);
+    *reinterpret_cast<uint2*>((value ? v_pages : k_pages) + cell[i] * p.hd + lane * 8) =
+        make_uint2(codes_of(v[i][0], v[i][1], v[i][2], v[i][3], k), codes_of(v[i][4], v[i][5], v[i][6], v[i][7], k));
+    if (lane == 0) (value ? v_scales : k_scales)[cell[i]] = k.s;
+  }
 }
 
-template <typename T, int LANES>
+template <typename T, int LANES, int R>
 __global__ void __launch_bounds__(256)
-int8_load_kernel(T* __restrict__ k_out, T* __restrict__ v_out, int64_t ld_k, int64_t ld_v, int vec, const int* __restrict__ row_seq,
-                 const int* __restrict__ row_pos, const int* __restrict__ table, int table_width, const int8_t* __restrict__ k_pages,
-                 const float* __restrict__ k_scales, const int8_t* __restrict__ v_pages, const float* __restrict__ v_scales, int n, int heads, int hd, int page) {
+int8_load_kernel(T* k_out, T* v_out, int64_t ld_k, int64_t ld_v, int vec, const Pages p, const int8_t* k_pages,
+                 const float* k_scales, const int8_t* v_pages, const float* v_scales, int n) {
+  constexpr int GROUPS = 256 / LANES;
   pdl_launch_dependents();
-  const int lane = threadIdx.x % LANES;
-  const int64_t item = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES, head = blockIdx.y >> 1;
+  const bool value = blockIdx.y & 1;
+  const int row0 = blockIdx.x * (GROUPS * R) + group;
   pdl_wait();
-  if (item >= (int64_t)n * heads * 2 || lane * 8 >= hd) return;
-  const Place p = place_of(item, heads, page, row_seq, row_pos, table, table_width);
-  const uint2 q = *reinterpret_cast<const uint2*>((p.value ? v_pages : k_pages) + p.cell * hd + lane * 8);
-  const float s = (p.value ? v_scales : k_scales)[p.cell];
-  float v[8];
+  if (lane * 8 >= p.hd) return;
+  uint2 q[R];
+  float s[R];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = (float)(int8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3))) * s;
-  store8((p.value ? v_out : k_out) + p.row * (p.value ? ld_v : ld_k) + (int64_t)p.head * hd + lane * 8, vec, v);
+  for (int i = 0; i < R; ++i) {
+    const int row = row0 + i * GROUPS;
+    if (row < n) {
+      const int64_t cell = p.cell(row, head);
+      q[i] = *reinterpret_cast<const uint2*>((value ? v_pages : k_pages) + cell * p.hd + lane * 8);
+      s[i] = (value ? v_scales : k_scales)[cell];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int row = row0 + i * GROUPS;
+    if (row >= n) continue;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)((e < 4 ? q[i].x : q[i].y) >> (8 * (e & 3))) * s[i];
+    store8((value ? v_out : k_out) + (int64_t)row * (value ? ld_v : ld_k) + (int64_t)head * p.hd + lane * 8, vec, v);
+  }
 }
 
 // f(lanes) with as many lanes as a row of hd entries takes, a power of two.
@@ -150,9 +162,19 @@ template <typename F> cudaError_t by_lanes(int hd, F f) {
 
 int check(const char* what, int n, int heads, int hd, int page, int table_width, const void* kp, const void* vp) {
   KVAD_REQUIRE(n > 0 && heads > 0 && page > 0 && table_width > 0, "%s: needs rows, heads and pages", what);
+  KVAD_REQUIRE(heads <= 32767, "%s: more heads than a launch takes", what);
   if (hd <= 0 || hd % 16 || hd > 256) KVAD_FAIL(KVAD_ERR_UNSUPPORTED, "%s: head sizes are multiples of 16 up to 256, not %d", what, hd);
   KVAD_REQUIRE(((reinterpret_cast<uintptr_t>(kp) | reinterpret_cast<uintptr_t>(vp)) & 15) == 0, "%s: pages must start on a 16-byte boundary", what);
   return KVAD_OK;
+}
+
+constexpr int MANY = 512;        // rows from which on a group of lanes takes four
+
+Pages pages(const int* row_seq, const int* row_pos, const int* table, int width, int heads, int hd, int page) {
+  int shift = -1;
+  if ((page & (page - 1)) == 0)
+    for (shift = 0; (1 << shift) < page;) ++shift;
+  return Pages{row_seq, row_pos, table, width, heads, hd, page, shift};
 }
 
 bool whole(const void* p, int64_t ld, int size) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (ld * size) % 16 == 0; }
@@ -166,16 +188,18 @@ KVAD_EXPORT int kvad_kv_store_int8(int dtype, const void* k_src, const void* v_s
   if (bad) return bad;
   const int size = dtype == KVAD_DTYPE_F32 ? 4 : 2;
   const int vec = whole(k_src, ld_src, size) && whole(v_src, ld_src, size);
+  const Pages p = pages(row_seq, row_pos, table, table_width, heads, hd, page);
   const cudaError_t e = by_lanes(hd, [&](auto lanes) {
     constexpr int L = decltype(lanes)::value;
-    const int64_t blocks = ((int64_t)n * heads * 2 + 256 / L - 1) / (256 / L);
-    if (blocks >= (1ll << 31)) return cudaErrorInvalidConfiguration;
-    auto launch = [&](auto kernel, auto* k, auto* v) {
-      return kvad_launch(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, k, v, ld_src, vec, row_seq, row_pos, table, table_width, k_pages, k_scales,
-                         v_pages, v_scales, n, heads, hd, page);
+    auto launch = [&](auto kernel, int r, auto* k, auto* v) {
+      return kvad_launch(kernel, dim3((unsigned)((n + 256 / L * r - 1) / (256 / L * r)), heads * 2), dim3(256), 0, stream, k, v, ld_src, vec, p, k_pages, k_scales,
+                         v_pages, v_scales, n);
     };
-    return dtype == KVAD_DTYPE_F32 ? launch(int8_store_kernel<float, L>, (const float*)k_src, (const float*)v_src)
-                                   : launch(int8_store_kernel<__nv_bfloat16, L>, (const __nv_bfloat16*)k_src, (const __nv_bfloat16*)v_src);
+    auto go = [&](auto* k, auto* v) {
+      using T = std::remove_cv_t<std::remove_pointer_t<decltype(k)>>;
+      return n >= MANY ? launch(int8_store_kernel<T, L, 4>, 4, k, v) : launch(int8_store_kernel<T, L, 1>, 1, k, v);
+    };
+    return dtype == KVAD_DTYPE_F32 ? go((const float*)k_src, (const float*)v_src) : go((const __nv_bfloat16*)k_src, (const __nv_bfloat16*)v_src);
   });
   if (e != cudaSuccess) KVAD_FAIL(KVAD_ERR_CUDA, "kv_store_int8: launch failed: %s", cudaGetErrorString(e));
   KVAD_CHECK_LAUNCH("kv_store_int8");
@@ -189,16 +213,18 @@ KVAD_EXPORT int kvad_kv_read_int8(int dtype, void* k_out, void* v_out, int64_t l
   if (bad) return bad;
   const int size = dtype == KVAD_DTYPE_F32 ? 4 : 2;
   const int vec = whole(k_out, ld_k, size) && whole(v_out, ld_v, size);
+  const Pages p = pages(row_seq, row_pos, table, table_width, heads, hd, page);
   const cudaError_t e = by_lanes(hd, [&](auto lanes) {
     constexpr int L = decltype(lanes)::value;
-    const int64_t blocks = ((int64_t)n * heads * 2 + 256 / L - 1) / (256 / L);
-    if (blocks >= (1ll << 31)) return cudaErrorInvalidConfiguration;
-    auto launch = [&](auto kernel, auto* k, auto* v) {
-      return kvad_launch(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, k, v, ld_k, ld_v, vec, row_seq, row_pos, table, table_width, k_pages, k_scales,
-                         v_pages, v_scales, n, heads, hd, page);
+    auto launch = [&](auto kernel, int r, auto* k, auto* v) {
+      return kvad_launch(kernel, dim3((unsigned)((n + 256 / L * r - 1) / (256 / L * r)), heads * 2), dim3(256), 0, stream, k, v, ld_k, ld_v, vec, p, k_pages, k_scales,
+                         v_pages, v_scales, n);
     };
-    return dtype == KVAD_DTYPE_F32 ? launch(int8_load_kernel<float, L>, (float*)k_out, (float*)v_out)
-                                   : launch(int8_load_kernel<__nv_bfloat16, L>, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out);
+    auto go = [&](auto* k, auto* v) {
+      using T = std::remove_pointer_t<decltype(k)>;
+      return n >= MANY ? launch(int8_load_kernel<T, L, 4>, 4, k, v) : launch(int8_load_kernel<T, L, 1>, 1, k, v);
+    };
+    return dtype == KVAD_DTYPE_F32 ? go((float*)k_out, (float*)v_out) : go((__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out);
   });
   if (e != cudaSuccess) KVAD_FAIL(KVAD_ERR_CUDA, "kv_read_int8: launch failed: %s", cudaGetErrorString(e));
   KVAD_CHECK_LAUNCH("kv_read_int8");

@@ -12,7 +12,9 @@
 // One pass: a row's entries stay in the registers of its threads from the sum through both reductions (mean square, maximum) to the
 // codes.  Sums, norms and scales are 32-bit; the only rounding to fewer bits is the code itself.
 // kvad_int8_read: codes back to numbers.
-#include "common.cuh"
+//
+// No pointer is __restrict__: what is promised not to change may be read before the wait for the kernel that writes it.
+#include "int8_codes.cuh"
 
 using namespace kvad;
 
@@ -65,9 +67,9 @@ template <int TPR> __device__ __forceinline__ uint32_t row_max(uint32_t v, float
 // TPR threads a row, 4 * V entries a thread at most.  VEC: four entries at a time (every row on a 4-entry boundary), else one.
 template <typename T, int NORM, int TPR, int V, bool VEC>
 __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
-int8_rows_kernel(const T* __restrict__ x, int64_t ld_x, const int* __restrict__ rows, const void* __restrict__ delta, int delta_f32, int64_t ld_delta,
-                 float mult, float* __restrict__ x_out, int64_t ld_out, const void* __restrict__ weight, const void* __restrict__ bias, int params_f32,
-                 int unit_offset, int8_t* __restrict__ codes, int64_t ld_codes, float* __restrict__ scales, int n, int width, float eps) {
+int8_rows_kernel(const T* x, int64_t ld_x, const int* rows, const void* delta, int delta_f32, int64_t ld_delta,
+                 float mult, float* x_out, int64_t ld_out, const void* weight, const void* bias, int params_f32,
+                 int unit_offset, int8_t* codes, int64_t ld_codes, float* scales, int n, int width, float eps) {
   constexpr int BLOCK = TPR < 128 ? 128 : TPR;
   __shared__ float scratch[TPR == 32 ? 1 : TPR / 32];
   // (what rows without a norm become may be weights, which the products fetch before they wait for the kernel before them: no early start there)
@@ -154,31 +156,22 @@ int8_rows_kernel(const T* __restrict__ x, int64_t ld_x, const int* __restrict__ 
     top = bits > top ? bits : top;
   }
   top = row_max<TPR>(top, scratch);
-  const bool finite = top < 0x7f800000u;
-  const float scale = finite ? __fmul_rn(__uint_as_float(top), 1.f / 127.f) : __uint_as_float(0x7fffffffu);
-  const bool some = finite && scale > 0.f;
-  if (t == 0) scales[r] = scale;
+  const Scale k = scale_of(top);
+  if (t == 0) scales[r] = k.s;
   int8_t* cr = codes + r * ld_codes;
 #pragma unroll
   for (int e = 0; e < 4 * V; e += VEC ? 4 : 1) {
     const int j = place(e);
     if (j < width) {
-      int c[4];
-#pragma unroll
-      for (int i = 0; i < (VEC ? 4 : 1); ++i) {
-        // (a scale below the smallest normal number is off by up to half: the quotient may then pass 127)
-        const float q = some ? __fdiv_rn(v[e + i], scale) : 0.f;
-        c[i] = __float2int_rn(fminf(fmaxf(q, -127.f), 127.f));
-      }
-      if (VEC) *reinterpret_cast<uint32_t*>(cr + j) = (c[0] & 0xff) | (c[1] & 0xff) << 8 | (c[2] & 0xff) << 16 | (uint32_t)(c[3] & 0xff) << 24;
-      else cr[j] = (int8_t)c[0];
+      if (VEC) *reinterpret_cast<uint32_t*>(cr + j) = codes_of(v[e], v[e + 1], v[e + 2], v[e + 3], k);
+      else cr[j] = (int8_t)code_of(v[e], k);
     }
   }
 }
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
-int8_read_kernel(const int8_t* __restrict__ codes, int64_t ld_codes, const float* __restrict__ scales, T* __restrict__ out, int64_t ld_out, int n, int width) {
+int8_read_kernel(const int8_t* codes, int64_t ld_codes, const float* scales, T* out, int64_t ld_out, int n, int width) {
   pdl_launch_dependents();
   const int per_row = VEC ? (width + 15) / 16 : width;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;

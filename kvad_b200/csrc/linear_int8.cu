@@ -67,9 +67,10 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, ui
 }
 
 // NT groups of eight rows.  Weights are the M side of the product (16 outputs), rows its N side.
+// (`a` is not __restrict__: what is promised not to change may be read before the wait for the kernel that writes it.)
 template <typename T, int EPI, int NT>
 __global__ void __launch_bounds__(FEW_WARPS * 32)
-linear_int8_few_kernel(const int8_t* __restrict__ a, int64_t lda, const int8_t* __restrict__ w, Out o, int M, int N, int K) {
+linear_int8_few_kernel(const int8_t* a, int64_t lda, const int8_t* __restrict__ w, Out o, int M, int N, int K) {
   __shared__ int part[FEW_WARPS][NT * 8][17];
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;

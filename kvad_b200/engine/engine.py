@@ -163,8 +163,9 @@ class Engine:
     # -- loading -------------------------------------------------------------------
     @classmethod
     def from_pretrained(cls, model_dir: str, dtype="bfloat16", *, device="cuda:0", max_tokens: int = 65536,
-                        max_seqs: Optional[int] = None, verbose: bool = False) -> "Engine":
-        """Loads a model folder (config.json + safetensors); the class is chosen by config.json."""
+                        max_seqs: Optional[int] = None, verbose: bool = False, int8: bool = False) -> "Engine":
+        """Loads a model folder (config.json + safetensors); the class is chosen by config.json.  `int8`: the blocks' products and the cache
+        in 8-bit codes with 32-bit scales (architectures of pre-norm blocks with plain attention: GPT-2)."""
         tdtype = parse_dtype(dtype)
         if not torch.cuda.is_available():
             raise KernelError("no CUDA device: kvad_b200 has no CPU path")
@@ -177,7 +178,11 @@ class Engine:
                     e = ckpt.entries.get(name)
                     return None if e is None else tuple(e.shape)
                 config = arch.with_checkpoint_shapes(config, shape_of)
-            model = Model(arch.plan(config))
+            plan = arch.plan(config)
+            if int8:
+                from ..models.int8 import int8_plan
+                plan = int8_plan(plan)
+            model = Model(plan)
             # compile (first call only) what this model's parts launch from, and no more, before the weights take time
             from ..csrc import build
             build.build_all(libraries_for(tdtype, model.kernel_families()), verbose=True)

@@ -230,7 +230,7 @@ _SIGNATURES = {
     },
     "attention_int8_prompt": {
         "kvad_attention_int8_prompt": [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
-                                       c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p],
+                                       c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
         "kvad_attention_int8_prompt_status": [],
         "kvad_attention_int8_prompt_test_hooks": [c_uint, c_int],
     },
@@ -1953,6 +1953,7 @@ class Ops:
         """Causal softmax attention of packed rows (each sequence's rows are its last positions; `max_new`: the longest run of them) over the paged cache
         of 8-bit codes (`kv_store_int8`).  A row sees the positions up to its own, or with a `window` the last so many and always the first
         `keep_first`.  Several query heads may share a key/value head.  Head sizes are multiples of 16 up to 256, pages hold 64 positions."""
+        global _launches
         _need_cuda(q, out, seq_starts, kv_lens, page_table, k_pages, k_scales, v_pages, v_scales)
         ld_q, ld_o = _rows_view(q, "attention queries"), _rows_view(out, "attention output")
         _, n_kv, page, hd = self._int8_pages("attention_int8", k_pages, k_scales, v_pages, v_scales)
@@ -1967,11 +1968,15 @@ class Ops:
         if (max_new > 1 and self.dtype == torch.bfloat16 and hd in self.INT8_PROMPT_HEAD_SIZES and page == 64 and n_heads % n_kv == 0 and n_heads // n_kv <= 128
                 and ld_q % 8 == 0 and ld_o % 8 == 0
                 and (q.data_ptr() | out.data_ptr() | k_pages.data_ptr() | v_pages.data_ptr() | k_scales.data_ptr() | v_scales.data_ptr()) % 16 == 0):
+            parts, part_pages = self.int8_parts(n, n_seqs, n_kv, n_heads // n_kv, page_table.shape[1], window, keep_first)
+            scratch = torch.empty(n * n_heads * parts * (hd + 2), dtype=torch.float32, device=q.device) if parts > 1 else None
             h = lib("attention_int8_prompt")
             _check(h.kvad_attention_int8_prompt(q.data_ptr(), ld_q, out.data_ptr(), ld_o, seq_starts.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(),
                                                 page_table.shape[1], k_pages.data_ptr(), k_scales.data_ptr(), v_pages.data_ptr(), v_scales.data_ptr(), n,
                                                 int(n_seqs), int(max_new), int(n_heads), n_kv, hd, page, float(scale), int(window or 0), int(keep_first or 0),
-                                                _stream()), h)
+                                                parts, part_pages, _ptr(scratch), _stream()), h)
+            if parts > 1:
+                _launches += 1          # the blocks of a row meet
             return
         splits, split_pages, warps, scratch = 1, 0, 4, None
         if max_new == 1:
@@ -1985,8 +1990,21 @@ class Ops:
                                      int(n_seqs), int(max_new), int(n_heads), n_kv, hd, page, float(scale), int(window or 0), int(keep_first or 0), splits,
                                      split_pages, warps, _ptr(scratch), _stream()), h)
         if splits > 1:
-            global _launches
             _launches += 1          # the blocks of a row and head meet
+
+    @staticmethod
+    def int8_parts(n_rows: int, n_seqs: int, n_kv: int, group: int, width: int, window: int = 0, keep_first: int = 0, n_sms: Optional[int] = None) -> tuple:
+        """Into how many parts prompt rows cut the pages they see, and pages a part: two blocks for every SM, eight pages a part at least, from 24 pages on.
+        (us whole and so: 330 rows of 8 heads of 128 on 2 behind 2500 positions 60, 36; 5 behind 8000 132, 23; 4096 rows of 8 heads of 128 87, 77; 1024 rows of
+        12 heads of 64, 16 pages, 25.0 and in two parts 26.3: joining costs what it saves.)"""
+        tokens = 2 * (128 // group)                 # of a block
+        reach = width if not window else min(width, -(-(window + tokens) // 64) + 1 + -(-keep_first // 64))
+        blocks = (n_rows // tokens + n_seqs) * n_kv
+        parts = min(2 * (n_sms or sm_count()) // blocks, reach // 8) if reach >= 24 else 1
+        if parts <= 1:
+            return 1, 0
+        pages = -(-reach // parts)
+        return -(-reach // pages), pages
 
     @staticmethod
     def int8_splits(items: int, reach: int, n_sms: Optional[int] = None) -> tuple:

@@ -1,0 +1,142 @@
+"""Parts that hold their weights, their inputs and what they keep per position in 8 bits.
+
+A row is codes of -127 .. 127 and a 32-bit scale, max|x| / 127 (`Ops.int8_rows`).  Weights are turned into such rows once, while loading, one
+scale an output; activations row by row on their way into each product - in the norm's pass where a norm comes before, in one of their own where
+heads' outputs or a feed-forward's inner rows go on; keys and values as they are written to the cache, one scale a position and head.  The
+products' sums are whole numbers; the residual stream, norms, scores, softmax weights and sums stay in 32-bit; queries and what comes out of a
+product that does not add into the stream have the engine's dtype.
+
+`pre_norm_int8`, `causal_attention_int8` and `dense_mlp_int8` take the parameters of the parts whose names they extend and ask for the same tensors
+(`models/int8.py` rewrites a plan in their terms); inputs of products are multiples of 16.
+"""
+from __future__ import annotations
+
+import torch
+
+from ..cache.layout import KVNeed
+from .attention import CausalSelfAttention
+from .base import PartSpec, register_part
+from .block import PreNormBlock
+from .feedforward import ACTIVATIONS, DenseMLP
+from .linear import Linear
+
+
+class Rows8:
+    """Rows of a step as codes and scales."""
+
+    def __init__(self, ctx, n: int, width: int):
+        self.codes = ctx.buffer((n, width), torch.int8)
+        self.scales = ctx.buffer((n,), torch.float32)
+
+    @property
+    def shape(self):
+        return self.codes.shape
+
+    @classmethod
+    def of(cls, ctx, x) -> "Rows8":
+        rows = cls(ctx, x.shape[0], x.shape[1])
+        ctx.ops.int8_rows(x, rows.codes, rows.scales)
+        return rows
+
+
+class Int8Linear(Linear):
+    """A `Linear` whose weight is held as codes `[out, in]` and a scale an output; it takes `Rows8`."""
+    kernel_families = ("int8",)
+
+    def __init__(self, prefix: str, in_features: int, out_features: int, **kw):
+        super().__init__(prefix, in_features, out_features, **kw)
+        if self.in_features % 16:
+            raise ValueError(f"8-bit products take inputs of a multiple of 16 entries, `{prefix}` has {in_features}")
+        self.codes = self.scales = None
+
+    def load_own(self, fetch):
+        from ..ops import Ops
+        weight = fetch(self.prefix + self.weight_name, transpose=self.stored == "in_out", keep_f32=True).contiguous()
+        self.codes = torch.empty(weight.shape, dtype=torch.int8, device=weight.device)
+        self.scales = torch.empty(weight.shape[0], dtype=torch.float32, device=weight.device)
+        Ops(weight.dtype).int8_rows(weight, self.codes, self.scales)
+        if self.has_bias:
+            self.bias = fetch(self.prefix + self.bias_name, keep_f32=True, optional=self.bias_optional)
+
+    def own_tensors(self):
+        return [t for t in (self.codes, self.scales, self.bias) if t is not None]
+
+    def forward(self, ctx, a: Rows8, out: torch.Tensor, epilogue: str = "store") -> torch.Tensor:
+        ctx.ops.linear_int8(a.codes, a.scales, self.codes, self.scales, self.bias, out, epilogue)
+        return out
+
+
+def _in_8_bits(linear: Linear) -> Int8Linear:
+    return Int8Linear(linear.prefix, linear.in_features, linear.out_features, bias=linear.has_bias, stored=linear.stored,
+                      bias_optional=linear.bias_optional, weight_name=linear.weight_name, bias_name=linear.bias_name)
+
+
+class Int8Attention(CausalSelfAttention):
+    kernel_families = ("int8",)
+
+    def __init__(self, prefix: str, width: int, n_heads: int, head_dim: int, score_scale: float, **kw):
+        super().__init__(prefix, width, n_heads, head_dim, score_scale, **kw)
+        if self.head_dim > 256:
+            raise ValueError(f"attention over an 8-bit cache takes heads of up to 256 entries, not {self.head_dim}")
+        self.qkv, self.out = _in_8_bits(self.qkv), _in_8_bits(self.out)
+
+    def cache_need(self):
+        return KVNeed(self.n_kv_heads, self.head_dim, self.window, int8=True)
+
+    def forward(self, ctx, h: Rows8, residual, call):
+        n, ops, view = h.shape[0], ctx.ops, ctx.kv(call.cache)
+        qkv = ctx.buffer((n, self.q_width + 2 * self.kv_width))
+        self.qkv.forward(ctx, h, qkv)
+        q, k, v = qkv[:, :self.q_width], qkv[:, self.q_width:self.q_width + self.kv_width], qkv[:, self.q_width + self.kv_width:]
+        if self.position is not None:
+            ctx.shared["rotary_head_dim"] = self.head_dim
+            self.position.rotate(ctx, q, k)
+        pages = (view.k_pages, view.k_scales, view.v_pages, view.v_scales)
+        if call.writes_cache:
+            ops.kv_store_int8(k, v, ctx.row_seq, ctx.row_pos, view.page_table, *pages)
+        mixed = ctx.buffer((n, self.q_width))
+        ops.attention_int8(q, mixed, ctx.seq_starts, ctx.kv_lens, ctx.n_seqs, ctx.batch.max_new, view.page_table, *pages, self.n_heads, self.score_scale,
+                           window=view.window or 0)
+        self.out.forward(ctx, Rows8.of(ctx, mixed), residual, "residual")
+
+
+class Int8MLP(DenseMLP):
+    kernel_families = ("int8",)
+
+    def __init__(self, prefix: str, width: int, hidden: int, activation: str, **kw):
+        super().__init__(prefix, width, hidden, activation, **kw)
+        self.up, self.down = _in_8_bits(self.up), _in_8_bits(self.down)
+
+    def forward(self, ctx, h: Rows8, residual):
+        hid = ctx.buffer((h.shape[0], self.hidden))
+        self.up.forward(ctx, h, hid, ACTIVATIONS[self.activation])
+        self.down.forward(ctx, Rows8.of(ctx, hid), residual, "residual")
+
+
+class Int8PreNormBlock(PreNormBlock):
+    """x += mixer(norm1(x)); x += ff(norm2(x)), the norms' rows in 8 bits."""
+    kernel_families = ("int8",)
+
+    def __init__(self, prefix: str, norm1: PartSpec, mixer: PartSpec, norm2: PartSpec, feed_forward: PartSpec, **kw):
+        super().__init__(prefix, norm1, mixer, norm2, feed_forward, **kw)
+        if self.norm1.affine() is None or self.norm2.affine() is None:
+            raise ValueError("pre_norm_int8 takes layer norms, and RMS norms with a weight that is stored as it is")
+
+    @staticmethod
+    def _normed(ctx, norm, x) -> Rows8:
+        gain, bias, centred, eps = norm.affine()
+        rows = Rows8(ctx, ctx.n_rows, x.shape[1])
+        if centred:
+            ctx.ops.layernorm_int8(x, gain, bias, eps, rows.codes, rows.scales)
+        else:
+            ctx.ops.rmsnorm_int8(x, gain, eps, rows.codes, rows.scales)
+        return rows
+
+    def forward(self, ctx, x, call):
+        self.mixer.forward(ctx, self._normed(ctx, self.norm1, x), x, call)
+        self.feed_forward.forward(ctx, self._normed(ctx, self.norm2, x), x)
+
+
+register_part("mixer", "causal_attention_int8", Int8Attention)
+register_part("feed_forward", "dense_mlp_int8", Int8MLP)
+register_part("block", "pre_norm_int8", Int8PreNormBlock)
