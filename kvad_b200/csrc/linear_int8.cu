@@ -6,7 +6,8 @@
 // and come by TMA in blocks of 128 entries of K (one row of the 128-byte swizzle); a CTA computes tiles of 128 x BN, one after another, the
 // epilogue of one under the products of the next (two accumulators).
 //
-// Few rows: a stream of weights.  A CTA has 16 outputs; its warps share K in pieces of 64 entries, of which a lane brings 16 contiguous
+// Few rows: a stream of weights, bound by their bytes (8 rows into 50257 outputs of 1600 entries: 18.9 us, 4.3 TB/s) and in small products by a launch and one
+// trip to memory (into 4800 outputs: 4.1 us).  A CTA has 16 outputs; its warps share K in pieces of 64 entries, of which a lane brings 16 contiguous
 // bytes of two outputs' weights straight into registers - mma.sync takes K in any order, so long as rows and weights agree on it.
 //
 // Every wait on an mbarrier is bounded; one that runs out raises a counter (kvad_linear_int8_status), and the CTA frees its tensor memory and returns.
@@ -59,7 +60,6 @@ __device__ __forceinline__ void put(const Out& o, int64_t at, float t) {
 // ---------------------------------------------------------------------------------------------------------------------------
 // Few rows
 // ---------------------------------------------------------------------------------------------------------------------------
-constexpr int FEW_WARPS = 8;
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -68,24 +68,23 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, ui
 
 // NT groups of eight rows.  Weights are the M side of the product (16 outputs), rows its N side.
 // (`a` is not __restrict__: what is promised not to change may be read before the wait for the kernel that writes it.)
-template <typename T, int EPI, int NT>
-__global__ void __launch_bounds__(FEW_WARPS * 32)
+template <typename T, int EPI, int NT, int WARPS, int U>
+__global__ void __launch_bounds__(WARPS * 32)
 linear_int8_few_kernel(const int8_t* a, int64_t lda, const int8_t* __restrict__ w, Out o, int M, int N, int K) {
-  __shared__ int part[FEW_WARPS][NT * 8][17];
+  __shared__ int part[WARPS][NT * 8][17];
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int n0 = blockIdx.x * 16;
   const int chunks = (K + 63) / 64;
-  constexpr int U = NT <= 2 ? 4 : 2;            // pieces of K a lane asks for at a time
   int acc[NT][4] = {};
   const int8_t* w0 = w + (int64_t)(n0 + g < N ? n0 + g : N - 1) * K + t * 16;
   const int8_t* w1 = w + (int64_t)(n0 + g + 8 < N ? n0 + g + 8 : N - 1) * K + t * 16;
   bool waited = false;
-  for (int c0 = warp; c0 < chunks; c0 += FEW_WARPS * U) {
-    int4 wa[U], wb[U];
+  for (int c0 = warp; c0 < chunks; c0 += WARPS * U) {
+    int4 wa[U], wb[U];                          // a lane asks for U pieces of K at a time
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int k = (c0 + u * FEW_WARPS) * 64;
+      const int k = (c0 + u * WARPS) * 64;
       wa[u] = wb[u] = make_int4(0, 0, 0, 0);
       if (k + t * 16 < K) {
         wa[u] = __ldg(reinterpret_cast<const int4*>(w0 + k));
@@ -98,7 +97,7 @@ linear_int8_few_kernel(const int8_t* a, int64_t lda, const int8_t* __restrict__ 
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int k = (c0 + u * FEW_WARPS) * 64 + t * 16;
+      const int k = (c0 + u * WARPS) * 64 + t * 16;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int m = nt * 8 + g;
@@ -118,12 +117,12 @@ linear_int8_few_kernel(const int8_t* a, int64_t lda, const int8_t* __restrict__ 
     part[warp][nt * 8 + 2 * t + 1][g + 8] = acc[nt][3];
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < NT * 8 * 16; i += FEW_WARPS * 32) {
+  for (int i = threadIdx.x; i < NT * 8 * 16; i += WARPS * 32) {
     const int m = i >> 4, j = i & 15, n = n0 + j;
     if (m >= M || n >= N) continue;
     int s = 0;
 #pragma unroll
-    for (int x = 0; x < FEW_WARPS; ++x) s += part[x][m][j];
+    for (int x = 0; x < WARPS; ++x) s += part[x][m][j];
     float y = (float)s * o.sa[m] * o.sw[n];
     if (o.bias != nullptr) y += load_param(o.bias, n, o.bias_f32);
     put<T, EPI>(o, (int64_t)m * o.ld + n, finish<EPI>(y));
@@ -140,9 +139,11 @@ template <int BN> struct Tile {
   static constexpr uint32_t A_BYTES = BM * BK, B_BYTES = BN * BK;
   static constexpr int STAGES_RAW = 192 * 1024 / (A_BYTES + B_BYTES);
   static constexpr int STAGES = STAGES_RAW > 8 ? 8 : STAGES_RAW;
-  static constexpr uint32_t OFF_SLAB = STAGES * (A_BYTES + B_BYTES);        // 4 KB an epilogue warp: 32 rows x 128 bytes of output on their way out by TMA
-  static constexpr uint32_t OFF_BAR = OFF_SLAB + 8 * 4096;
-  static constexpr size_t SMEM = OFF_BAR + (2 * STAGES + 4) * 8 + 16 + 1024;
+  static constexpr uint32_t OFF_SLAB = STAGES * (A_BYTES + B_BYTES);        // two of 2 KB an epilogue warp: 32 rows x 64 bytes of output on their way out by TMA
+  static constexpr uint32_t OFF_COLS = OFF_SLAB + 8 * 4096;                 // a tile's scales and bias, an output each
+  static constexpr uint32_t OFF_BAR = OFF_COLS + 2 * BN * 4;
+  static constexpr size_t SMEM = OFF_BAR + (2 * STAGES + 4) * 8 + 16;
+  static_assert(SMEM <= 227 * 1024, "an SM's shared memory");
 };
 
 // Whole-number products of 8-bit codes with a 32-bit accumulator: both operands signed, both K-major.
@@ -158,36 +159,33 @@ __device__ __forceinline__ void umma_i8(uint32_t d, uint64_t a_desc, uint64_t b_
       ::"r"(d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(zero) : "memory");
 }
 
-// Sixteen columns of a row from tensor memory, there when the statement is over.  (One statement for the load and the wait: between two, the compiler is free to work on
-// registers that are still on their way.)
-__device__ __forceinline__ void tmem_read16(uint32_t addr, float (&v)[16]) {
-  uint32_t r[16];
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+// Asks for columns of a row in tensor memory, and waits for them.  (The registers go through the wait, so that nothing that works on them comes before it.)
+__device__ __forceinline__ void tmem_ask(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                : "r"(addr) : "memory");
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_arrived(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               : : "memory");
+}
+__device__ __forceinline__ void tmem_ask(uint32_t addr, uint32_t (&r)[32]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+               : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tmem_arrived(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               : : "memory");
 }
 
-// Sixteen consecutive entries of a vector from `n` on, zeros beyond N.
-__device__ __forceinline__ void load16(const float* p, int n, int N, float* v) {
-  if (n + 16 <= N && (reinterpret_cast<uintptr_t>(p + n) & 15) == 0) {
+// A row's COLS consecutive outputs where TMA cannot take them (a base or row stride off 16 bytes).
+template <typename T, int EPI, int COLS>
+__device__ __forceinline__ void put_all(const Out& o, int row, int n, int N, const float (&v)[COLS]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float4 q = __ldg(reinterpret_cast<const float4*>(p + n) + i);
-      v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = n + i < N ? __ldg(p + n + i) : 0.f;
-  }
-}
-
-// One row's sixteen consecutive outputs where TMA cannot take them (a base or row stride off 16 bytes).
-template <typename T, int EPI>
-__device__ __forceinline__ void put16(const Out& o, int row, int n, int N, const float* v) {
-#pragma unroll
-  for (int j = 0; j < 16; ++j)
+  for (int j = 0; j < COLS; ++j)
     if (n + j < N) put<T, EPI>(o, (int64_t)row * o.ld + n + j, v[j]);
 }
 
@@ -198,8 +196,7 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   using L = Tile<BN>;
   constexpr int STAGES = L::STAGES;
   constexpr uint32_t TMEM = 2 * BN;             // two accumulators (a power of two)
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* a_tiles = smem;
   uint8_t* b_tiles = smem + STAGES * L::A_BYTES;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
@@ -207,7 +204,9 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   uint64_t* acc_full = empty + STAGES;          // [2] the accumulator is complete
   uint64_t* acc_empty = acc_full + 2;           // [2] the eight epilogue warps have read it
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
-  __shared__ int gave_up;
+  volatile uint32_t* gave_up = tmem_slot + 1;
+  float* col_scale = reinterpret_cast<float*>(smem + L::OFF_COLS);
+  float* col_bias = col_scale + BN;
 
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -224,7 +223,7 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], 8);
     }
-    gave_up = 0;
+    *gave_up = (smem_u32(smem) & 1023) != 0;      // (the swizzle's rows start on 1024 bytes; the memory is asked for so)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -233,7 +232,7 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  bool ok = true;
+  bool ok = *gave_up == 0;
 
   if (warp == 0) {
     if (lane == 0) {
@@ -290,74 +289,82 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
       if (ok && one) umma_commit(&acc_full[buf]);
     }
   } else {
-    const int quarter = warp & 3, half = warp >= 6 ? 1 : 0;       // two warps share a quarter of the lanes and take its slabs in turn
+    const int quarter = warp & 3, half = warp >= 6 ? 1 : 0;       // two warps share a quarter of the lanes and take its pieces of columns in turn
     constexpr bool F32_OUT = EPI == EPI_RESIDUAL || EPI == EPI_STORE_F32 || std::is_same<T, float>::value;
-    constexpr int SLAB = F32_OUT ? 32 : 64;     // 128 bytes of output a row
-    uint8_t* slab = smem + L::OFF_SLAB + (warp - 2) * 4096;
-    bool used = false;
-    int lt = 0;
+    constexpr int COLS = F32_OUT ? 16 : 32, PIECES = BN / COLS / 2;       // 64 bytes of output a row
+    uint8_t* slabs = smem + L::OFF_SLAB + (warp - 2) * 4096;
+    int lt = 0, sent = 0;
     pdl_wait();
-    for (int t = blockIdx.x; t < n_tiles && ok; t += gridDim.x, ++lt) {
+    for (int t = blockIdx.x; t < n_tiles; t += gridDim.x, ++lt) {
       const int n0 = t % tiles_n * BN, m0 = t / tiles_n * BM, buf = lt & 1;
       const int row = m0 + quarter * 32 + lane;
       const float sa = row < M ? o.sa[row] : 0.f;
-      if (!mbar_wait(&acc_full[buf], (lt >> 1) & 1)) { ok = false; break; }
+      // the tile's scales and bias, while its products run
+      if (lt > 0) asm volatile("bar.sync 1, 256;" ::: "memory");         // the eight warps are done with those of the last
+      {
+        const int j = threadIdx.x - 64;
+        if (j < BN) {
+          col_scale[j] = n0 + j < N ? o.sw[n0 + j] : 0.f;
+          col_bias[j] = o.bias != nullptr && n0 + j < N ? load_param(o.bias, n0 + j, o.bias_f32) : 0.f;
+        }
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (ok) ok = mbar_wait(&acc_full[buf], (lt >> 1) & 1);             // (a warp whose wait runs out still meets the others above)
+      if (!ok) continue;
       tc_fence_after();
-      const uint32_t acc = tmem + (uint32_t)(buf * BN) + ((uint32_t)(quarter * 32) << 16);
-#pragma unroll 1
-      for (int c0 = half * SLAB; c0 < BN; c0 += 2 * SLAB) {
-        if (n0 + c0 >= N) break;
-        if (tma_out && used) {                  // the slab's last journey has been read
-          if (lane == 0) bulk_wait_read();
+      const uint32_t acc = tmem + (uint32_t)(buf * BN) + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * COLS);
+      const int columns = min(BN, N - n0);
+      uint32_t r[2][COLS];
+      tmem_ask(acc, r[0]);
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p) {
+        const int c = (2 * p + half) * COLS;
+        tmem_arrived(r[p & 1]);
+        if (p + 1 < PIECES) tmem_ask(acc + (uint32_t)((p + 1) * 2 * COLS), r[(p + 1) & 1]);      // the next piece comes while this one is worked on
+        if (c >= columns) continue;
+        float v[COLS];
+#pragma unroll
+        for (int j = 0; j < COLS; j += 4) {
+          const float4 s4 = *reinterpret_cast<const float4*>(col_scale + c + j), b4 = *reinterpret_cast<const float4*>(col_bias + c + j);
+          v[j] = finish<EPI>(fmaf((float)(int)r[p & 1][j] * sa, s4.x, b4.x));
+          v[j + 1] = finish<EPI>(fmaf((float)(int)r[p & 1][j + 1] * sa, s4.y, b4.y));
+          v[j + 2] = finish<EPI>(fmaf((float)(int)r[p & 1][j + 2] * sa, s4.z, b4.z));
+          v[j + 3] = finish<EPI>(fmaf((float)(int)r[p & 1][j + 3] * sa, s4.w, b4.w));
+        }
+        if (!tma_out) {
+          if (row < M) put_all<T, EPI, COLS>(o, row, n0 + c, N, v);
+          continue;
+        }
+        uint8_t* slab = slabs + (sent & 1) * 2048;
+        if (sent >= 2) {                        // its journey before has been read
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
           __syncwarp();
         }
-        used = true;
+        ++sent;
 #pragma unroll
-        for (int cc = 0; cc < SLAB; cc += 16) {
-          float v[16], s[16];
-          load16(o.sw, n0 + c0 + cc, N, s);
-          tmem_read16(acc + (uint32_t)(c0 + cc), v);
-#pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = (float)__float_as_int(v[j]) * sa * s[j];
-          if (o.bias != nullptr) {
-            if (o.bias_f32) {
-              load16(reinterpret_cast<const float*>(o.bias), n0 + c0 + cc, N, s);
-            } else {
-#pragma unroll
-              for (int j = 0; j < 16; ++j) s[j] = n0 + c0 + cc + j < N ? load_param(o.bias, n0 + c0 + cc + j, 0) : 0.f;
-            }
-#pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] += s[j];
-          }
-#pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = finish<EPI>(v[j]);
-          if (!tma_out) {
-            if (row < M) put16<T, EPI>(o, row, n0 + c0 + cc, N, v);
-          } else if (F32_OUT) {
-#pragma unroll
-            for (int j = 0; j < 16; j += 4)
-              *reinterpret_cast<float4*>(slab + lane * 128 + ((((cc + j) >> 2) ^ (lane & 7)) << 4)) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+        for (int q = 0; q < 4; ++q) {           // 16-byte pieces of the row's 64, swizzled
+          uint4 w;
+          if (F32_OUT) {
+            w = make_uint4(__float_as_uint(v[4 * q]), __float_as_uint(v[4 * q + 1]), __float_as_uint(v[4 * q + 2]), __float_as_uint(v[4 * q + 3]));
           } else {
+            uint32_t e[4];
 #pragma unroll
-            for (int j = 0; j < 16; j += 8) {
-              uint32_t q[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                __nv_bfloat162 p = __floats2bfloat162_rn(v[j + 2 * e], v[j + 2 * e + 1]);
-                q[e] = *reinterpret_cast<uint32_t*>(&p);
-              }
-              *reinterpret_cast<uint4*>(slab + lane * 128 + ((((cc + j) >> 3) ^ (lane & 7)) << 4)) = make_uint4(q[0], q[1], q[2], q[3]);
+            for (int i = 0; i < 4; ++i) {
+              __nv_bfloat162 two = __floats2bfloat162_rn(v[8 * q + 2 * i], v[8 * q + 2 * i + 1]);
+              e[i] = *reinterpret_cast<uint32_t*>(&two);
             }
+            w = make_uint4(e[0], e[1], e[2], e[3]);
           }
+          *reinterpret_cast<uint4*>(slab + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) = w;
         }
-        if (tma_out) {
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0 && m0 + quarter * 32 < M) {
-            if (EPI == EPI_RESIDUAL) tma_reduce_add_2d(&map_out, slab, n0 + c0, m0 + quarter * 32);
-            else tma_store_2d(&map_out, slab, n0 + c0, m0 + quarter * 32);
-            bulk_commit();
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+          if (m0 + quarter * 32 < M) {
+            if (EPI == EPI_RESIDUAL) tma_reduce_add_2d(&map_out, slab, n0 + c, m0 + quarter * 32);
+            else tma_store_2d(&map_out, slab, n0 + c, m0 + quarter * 32);
           }
+          bulk_commit();
         }
       }
       tc_fence_before();
@@ -366,11 +373,11 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     }
     if (lane == 0) bulk_wait_all();
   }
-  if (!ok) gave_up = 1;
+  if (!ok) *gave_up = 1;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (gave_up) outlast_what_is_in_flight();
+  if (*gave_up) outlast_what_is_in_flight();
   if (warp == 1) {
     __syncwarp();
     tmem_dealloc(tmem, TMEM);
@@ -387,13 +394,13 @@ int sm_count() {
   return n;
 }
 
-// A matrix whose rows lie ld entries apart, `box_rows` x 128 bytes a copy.
-int tensor_map(const void* p, CUtensorMapDataType type, int size, int64_t ld, int rows, int cols, int box_rows, CUtensorMap* map) {
+// A matrix whose rows lie ld entries apart, `box_rows` x `box_bytes` (64 or 128) a copy, swizzled within them.
+int tensor_map(const void* p, CUtensorMapDataType type, int size, int64_t ld, int rows, int cols, int box_rows, int box_bytes, CUtensorMap* map) {
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) KVAD_FAIL(KVAD_ERR_CUDA, "linear_int8: the driver does not offer cuTensorMapEncodeTiled");
   cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld * size};
-  cuuint32_t box[2] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows}, elem[2] = {1, 1};
-  CUresult r = fn(map, type, 2, const_cast<void*>(p), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  cuuint32_t box[2] = {(cuuint32_t)(box_bytes / size), (cuuint32_t)box_rows}, elem[2] = {1, 1};
+  CUresult r = fn(map, type, 2, const_cast<void*>(p), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) KVAD_FAIL(KVAD_ERR_CUDA, "linear_int8: cuTensorMapEncodeTiled failed (%d) for [%d, %d] entries, %lld apart", (int)r, rows, cols, (long long)ld);
   return KVAD_OK;
@@ -403,13 +410,13 @@ template <typename T, int EPI, int BN>
 int many(const int8_t* a, int64_t lda, const int8_t* w, const Out& o, int M, int N, int K, cudaStream_t stream) {
   using L = Tile<BN>;
   CUtensorMap ma, mw, mo;
-  int rc = tensor_map(a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, lda, M, K, BM, &ma);
-  if (rc == KVAD_OK) rc = tensor_map(w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, N, K, BN, &mw);
+  int rc = tensor_map(a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, lda, M, K, BM, 128, &ma);
+  if (rc == KVAD_OK) rc = tensor_map(w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, N, K, BN, 128, &mw);
   if (rc != KVAD_OK) return rc;
   constexpr bool f32_out = EPI == EPI_RESIDUAL || EPI == EPI_STORE_F32 || std::is_same<T, float>::value;
   constexpr int size = f32_out ? 4 : 2;
   const int tma_out = (o.ld * size) % 16 == 0 && (reinterpret_cast<uintptr_t>(o.p) & 15) == 0;
-  if (tma_out) rc = tensor_map(o.p, f32_out ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, size, o.ld, M, N, 32, &mo);
+  if (tma_out) rc = tensor_map(o.p, f32_out ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, size, o.ld, M, N, 32, 64, &mo);
   else mo = ma;
   if (rc != KVAD_OK) return rc;
   auto kernel = linear_int8_kernel<T, EPI, BN>;
@@ -429,11 +436,19 @@ int many(const int8_t* a, int64_t lda, const int8_t* w, const Out& o, int M, int
   return KVAD_OK;
 }
 
+// Up to 16 rows the stream of weights is the faster one, beyond it the tensor cores (us, bfloat16, sets of inputs larger than the L2 in turn):
+//   4800 outputs of 1600 entries: 8 rows 4.1 against 5.9, 16 rows 4.6 against 6.2, 32 rows 6.9 against 5.9;  8192 of 4096: 16 rows 12.0 against 14.9.
+constexpr int FEW_MAX = 16;
+// With inputs longer than this and no more blocks than SMs, a block's sixteen warps ask for all of up to 8192 entries at once; else eight warps for 2048
+// (8 rows of 6400 entries into 1600 outputs: 5.5 us against 7.9; with as many registers a thread, 4800 outputs of 1600 entries take 6.8 us against 4.1).
+constexpr int LONG = 2048;
+
 template <typename T, int EPI>
 int few(const int8_t* a, int64_t lda, const int8_t* w, const Out& o, int M, int N, int K, cudaStream_t stream) {
-  auto go = [&](auto kernel) { return kvad_launch(kernel, dim3((N + 15) / 16), dim3(FEW_WARPS * 32), 0, stream, a, lda, w, o, M, N, K); };
-  const cudaError_t e = M <= 8 ? go(linear_int8_few_kernel<T, EPI, 1>) : M <= 16 ? go(linear_int8_few_kernel<T, EPI, 2>)
-                        : M <= 32 ? go(linear_int8_few_kernel<T, EPI, 4>) : go(linear_int8_few_kernel<T, EPI, 8>);
+  auto go = [&](auto kernel, int warps) { return kvad_launch(kernel, dim3((N + 15) / 16), dim3(warps * 32), 0, stream, a, lda, w, o, M, N, K); };
+  const cudaError_t e = K > LONG && (N + 15) / 16 <= sm_count()
+      ? (M <= 8 ? go(linear_int8_few_kernel<T, EPI, 1, 16, 8>, 16) : go(linear_int8_few_kernel<T, EPI, 2, 16, 8>, 16))
+      : (M <= 8 ? go(linear_int8_few_kernel<T, EPI, 1, 8, 4>, 8) : go(linear_int8_few_kernel<T, EPI, 2, 8, 4>, 8));
   if (e != cudaSuccess) KVAD_FAIL(KVAD_ERR_CUDA, "linear_int8: launch failed: %s", cudaGetErrorString(e));
   return KVAD_OK;
 }
@@ -451,8 +466,6 @@ int tile_width(int M, int N) {
   return best;
 }
 
-constexpr int FEW_MAX = 64;
-
 template <typename T, int EPI>
 int go(const int8_t* a, int64_t lda, const int8_t* w, const Out& o, int M, int N, int K, int form, cudaStream_t stream) {
   if (form == 1 || (form == 0 && M <= FEW_MAX)) return few<T, EPI>(a, lda, w, o, M, N, K, stream);
@@ -463,7 +476,7 @@ int go(const int8_t* a, int64_t lda, const int8_t* w, const Out& o, int M, int N
 
 }  // namespace
 
-// `form`: 0: by the sizes; 1: the kernel of few rows (at most 64); 64, 128, 256: the kernel of many rows with tiles so wide.
+// `form`: 0: by the sizes; 1: the kernel of few rows (at most 16); 64, 128, 256: the kernel of many rows with tiles so wide.
 KVAD_EXPORT int kvad_linear_int8(int dtype, const int8_t* a, int64_t lda, const float* sa, const int8_t* w, const float* sw, const void* bias, int bias_f32,
                                  void* out, int64_t ldo, int M, int N, int K, int epi, int form, cudaStream_t stream) {
   KVAD_REQUIRE(M > 0 && N > 0 && K > 0, "linear_int8: needs rows, outputs and inputs, got %d, %d, %d", M, N, K);
