@@ -7,9 +7,10 @@
 //
 // so a position takes head size + 4 bytes a head, where bfloat16 takes 2 * head size.
 //
-// A group of lanes (a power of two, head size / 8 at least) has one row: a lane brings eight entries, the group's maximum is a few shuffles, and
-// the codes leave as eight bytes a lane.  A block has one head's keys or values of so many rows, four of them a group where there are many, all asked for before the
-// first is worked on.  Bound by memory: 2 * (entry + 1) bytes a code, counting both directions.
+// A group of lanes (a power of two, head size / 8 at least) has one row, and of it one head's keys or values, or four heads' where there are many rows: a lane
+// brings eight entries, the group's maximum is a few shuffles, and the codes leave as eight bytes a lane.  Where a row goes is looked up once for the four heads
+// (a chain of two trips to memory), and all their entries are asked for before the first is worked on.  Bound by memory, entry + 1 bytes
+// a code: 26289 bfloat16 rows of 8 heads of 128 are stored in 41 us (3.9 TB/s; four rows of one head a group: 79) and read in 30 (5.5 TB/s).
 //
 // No pointer is __restrict__: what is promised not to change may be read before the wait for the kernel that writes it.
 #include <type_traits>
@@ -82,39 +83,36 @@ struct Pages {
   }
 };
 
+// blockIdx.y: so many heads, blockIdx.z: their keys (0) or values (1).  Addresses step from head to head: worked out a head, they are half of the instructions.
 template <typename T, int LANES, int R>
 __global__ void __launch_bounds__(256)
 int8_store_kernel(const T* k_src, const T* v_src, int64_t ld_src, int vec, const Pages p, int8_t* k_pages,
                   float* k_scales, int8_t* v_pages, float* v_scales, int n) {
-  constexpr int GROUPS = 256 / LANES;
   pdl_launch_dependents();
-  const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES, head = blockIdx.y >> 1;
-  const bool value = blockIdx.y & 1, in = lane * 8 < p.hd;
-  const T* src = (value ? v_src : k_src) + (int64_t)head * p.hd + lane * 8;
-  const int row0 = blockIdx.x * (GROUPS * R) + group;
+  const int lane = threadIdx.x % LANES, row = blockIdx.x * (256 / LANES) + threadIdx.x / LANES, head = blockIdx.y * R;
+  const int heads = row < n && lane * 8 < p.hd ? min(R, p.heads - head) : 0;
+  const T* src = (blockIdx.z ? v_src : k_src) + row * ld_src + (head * p.hd + lane * 8);
   pdl_wait();
   float v[R][8] = {};
-  int64_t cell[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    if (i < heads) load8(src + i * p.hd, vec, v[i]);
+  const int64_t cell = heads > 0 ? p.cell(row, head) : 0;
+  int8_t* to = (blockIdx.z ? v_pages : k_pages) + cell * p.hd + lane * 8;
+  float* scale = (blockIdx.z ? v_scales : k_scales) + cell;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    const int row = row0 + i * GROUPS;
-    if (row < n) {
-      if (in) load8(src + row * ld_src, vec, v[i]);
-      cell[i] = p.cell(row, head);
-    }
-  }
+    float most = 0.f;
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    uint32_t top = 0;
+    for (int e = 0; e < 8; ++e) most = max_abs(most, v[i][e]);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[i][e]) & 0x7fffffffu);
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (!in || row0 + i * GROUPS >= n) continue;
-    const Scale k = scale_of(top);
-    *reinterpret_cast<uint2*>((value ? v_pages : k_pages) + cell[i] * p.hd + lane * 8) =
-        make_uint2(codes_of(v[i][0], v[i][1], v[i][2], v[i][3], k), codes_of(v[i][4], v[i][5], v[i][6], v[i][7], k));
-    if (lane == 0) (value ? v_scales : k_scales)[cell[i]] = k.s;
+    for (int o = LANES / 2; o > 0; o >>= 1) most = max_abs(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (i >= heads) continue;
+    const Scale k = scale_of(__float_as_uint(most));
+    *reinterpret_cast<uint2*>(to) = make_uint2(codes_of(v[i][0], v[i][1], v[i][2], v[i][3], k), codes_of(v[i][4], v[i][5], v[i][6], v[i][7], k));
+    if (lane == 0) *scale = k.s;
+    to += p.page * p.hd;
+    scale += p.page;
   }
 }
 
@@ -122,32 +120,30 @@ template <typename T, int LANES, int R>
 __global__ void __launch_bounds__(256)
 int8_load_kernel(T* k_out, T* v_out, int64_t ld_k, int64_t ld_v, int vec, const Pages p, const int8_t* k_pages,
                  const float* k_scales, const int8_t* v_pages, const float* v_scales, int n) {
-  constexpr int GROUPS = 256 / LANES;
   pdl_launch_dependents();
-  const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES, head = blockIdx.y >> 1;
-  const bool value = blockIdx.y & 1;
-  const int row0 = blockIdx.x * (GROUPS * R) + group;
+  const int lane = threadIdx.x % LANES, row = blockIdx.x * (256 / LANES) + threadIdx.x / LANES, head = blockIdx.y * R;
   pdl_wait();
-  if (lane * 8 >= p.hd) return;
+  if (row >= n || lane * 8 >= p.hd) return;
+  const int heads = min(R, p.heads - head);
+  const int64_t cell = p.cell(row, head);
+  const int8_t* from = (blockIdx.z ? v_pages : k_pages) + cell * p.hd + lane * 8;
+  const float* scale = (blockIdx.z ? v_scales : k_scales) + cell;
+  T* out = (blockIdx.z ? v_out : k_out) + row * (blockIdx.z ? ld_v : ld_k) + (head * p.hd + lane * 8);
   uint2 q[R];
   float s[R];
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const int row = row0 + i * GROUPS;
-    if (row < n) {
-      const int64_t cell = p.cell(row, head);
-      q[i] = *reinterpret_cast<const uint2*>((value ? v_pages : k_pages) + cell * p.hd + lane * 8);
-      s[i] = (value ? v_scales : k_scales)[cell];
+  for (int i = 0; i < R; ++i)
+    if (i < heads) {
+      q[i] = *reinterpret_cast<const uint2*>(from + i * (p.page * p.hd));
+      s[i] = scale[i * p.page];
     }
-  }
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    const int row = row0 + i * GROUPS;
-    if (row >= n) continue;
+    if (i >= heads) continue;
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)((e < 4 ? q[i].x : q[i].y) >> (8 * (e & 3))) * s[i];
-    store8((value ? v_out : k_out) + (int64_t)row * (value ? ld_v : ld_k) + (int64_t)head * p.hd + lane * 8, vec, v);
+    store8(out + i * p.hd, vec, v);
   }
 }
 
@@ -168,7 +164,7 @@ int check(const char* what, int n, int heads, int hd, int page, int table_width,
   return KVAD_OK;
 }
 
-constexpr int MANY = 512;        // rows from which on a group of lanes takes four
+constexpr int MANY = 512;        // rows from which on a group of lanes takes four heads of its row
 
 Pages pages(const int* row_seq, const int* row_pos, const int* table, int width, int heads, int hd, int page) {
   int shift = -1;
@@ -192,7 +188,7 @@ KVAD_EXPORT int kvad_kv_store_int8(int dtype, const void* k_src, const void* v_s
   const cudaError_t e = by_lanes(hd, [&](auto lanes) {
     constexpr int L = decltype(lanes)::value;
     auto launch = [&](auto kernel, int r, auto* k, auto* v) {
-      return kvad_launch(kernel, dim3((unsigned)((n + 256 / L * r - 1) / (256 / L * r)), heads * 2), dim3(256), 0, stream, k, v, ld_src, vec, p, k_pages, k_scales,
+      return kvad_launch(kernel, dim3((unsigned)((n + 256 / L - 1) / (256 / L)), (heads + r - 1) / r, 2), dim3(256), 0, stream, k, v, ld_src, vec, p, k_pages, k_scales,
                          v_pages, v_scales, n);
     };
     auto go = [&](auto* k, auto* v) {
@@ -217,7 +213,7 @@ KVAD_EXPORT int kvad_kv_read_int8(int dtype, void* k_out, void* v_out, int64_t l
   const cudaError_t e = by_lanes(hd, [&](auto lanes) {
     constexpr int L = decltype(lanes)::value;
     auto launch = [&](auto kernel, int r, auto* k, auto* v) {
-      return kvad_launch(kernel, dim3((unsigned)((n + 256 / L * r - 1) / (256 / L * r)), heads * 2), dim3(256), 0, stream, k, v, ld_k, ld_v, vec, p, k_pages, k_scales,
+      return kvad_launch(kernel, dim3((unsigned)((n + 256 / L - 1) / (256 / L)), (heads + r - 1) / r, 2), dim3(256), 0, stream, k, v, ld_k, ld_v, vec, p, k_pages, k_scales,
                          v_pages, v_scales, n);
     };
     auto go = [&](auto* k, auto* v) {

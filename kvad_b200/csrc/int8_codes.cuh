@@ -1,39 +1,52 @@
 // Numbers to 8-bit codes: c = x / s rounded to the nearest integer, halves to the even one, -127 .. 127, with s = max|x| / 127 of the row.
 //
-// The code is that of the correctly rounded quotient, which is what a reader of the definition computes; a division takes ten times a product, so the product with
-// 1 / s decides wherever it is not within 2^-10 of a half (it is off by less than 2^-15), and the division where it is.
+// The code is that of the correctly rounded quotient, which is what a reader of the definition computes: where x is half the row's largest entry the quotient is
+// 63.5, so halves are no rare event.  It takes three operations an entry (Markstein's theorem, IBM Journal of Research and Development 34, 1990): with y = 1 / s
+// correctly rounded and q = x y, which is within a unit in the last place of x / s, the remainder r = x - q s is exact and q + r y the correctly rounded quotient,
+// so long as r does not leave the normal numbers; rows whose scale is below 2^-90 are divided by the division.  (A product that leaves what is near a half
+// to a division takes 16384 rows of 4096 bfloat16 entries 1.5 times as long: of a warp's words of four codes a third have such an entry.)
 #pragma once
 #include "common.cuh"
 
 namespace kvad {
 
 struct Scale {
-  float s, inverse;      // inverse 0: a row without codes (zeros, or a number that is not finite)
-  bool small;            // s is below the smallest normal number: divisions throughout
+  float s, inverse;      // inverse 0: a row of zeros
+  uint32_t keep;         // 0: a row that holds a number that is not finite has codes 0
+  bool divide;
 };
+
+// The larger magnitude, NaN where either is; a row's largest says as well whether all of it is finite.
+__device__ __forceinline__ float max_abs(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+  return r;
+}
 
 // `top`: the bits of the row's largest magnitude; NaN and infinity are above every finite number.
 __device__ __forceinline__ Scale scale_of(uint32_t top) {
   Scale r;
   const bool finite = top < 0x7f800000u;
   r.s = finite ? __fmul_rn(__uint_as_float(top), 1.f / 127.f) : __uint_as_float(0x7fffffffu);
-  r.small = r.s < 1.17549435e-38f;
-  r.inverse = finite && r.s > 0.f ? __fdividef(1.f, r.small ? 1.f : r.s) : 0.f;
+  r.divide = r.s < 0x1p-90f && r.s > 0.f;
+  r.inverse = finite && r.s > 0.f ? __frcp_rn(r.s) : 0.f;
+  r.keep = finite ? 0xffffffffu : 0u;
   return r;
 }
 
-// The code of one number, in the lowest byte.
-__device__ __forceinline__ uint32_t code_of(float x, const Scale& k) {
-  constexpr float M = 12582912.f;               // 1.5 x 2^23: what is added to it is rounded to a whole number, which its lowest bits then are
-  if (k.inverse == 0.f) return 0u;
-  const float q = x * k.inverse, m = q + M;
-  if (!k.small && fabsf(q - (m - M)) <= 0.5f - 0x1p-10f) return __float_as_uint(m);
-  return __float_as_uint(fminf(fmaxf(__fdiv_rn(x, k.s), -127.f), 127.f) + M);
+// x / s and the whole number next to it, which the lowest byte of the result holds: 1.5 x 2^23 leaves no places behind the point.
+__device__ __forceinline__ uint32_t code_bits(float x, const Scale& k) {
+  const float q = x * k.inverse;
+  return __float_as_uint(fmaf(fmaf(-q, k.s, x), k.inverse, q) + 12582912.f);
 }
+__device__ __noinline__ uint32_t code_divided(float x, float s) { return __float_as_uint(__fdiv_rn(x, s) + 12582912.f) & 0xffu; }
+
+// The code of one number, in the lowest byte.
+__device__ __forceinline__ uint32_t code_of(float x, const Scale& k) { return k.divide ? code_divided(x, k.s) : code_bits(x, k) & k.keep & 0xffu; }
 // Four numbers' codes in a word.
 __device__ __forceinline__ uint32_t codes_of(float a, float b, float c, float d, const Scale& k) {
-  const uint32_t lo = __byte_perm(code_of(a, k), code_of(b, k), 0x0040), hi = __byte_perm(code_of(c, k), code_of(d, k), 0x0040);
-  return __byte_perm(lo, hi, 0x5410);
+  if (k.divide) return code_of(a, k) | code_of(b, k) << 8 | code_of(c, k) << 16 | code_of(d, k) << 24;
+  return __byte_perm(__byte_perm(code_bits(a, k), code_bits(b, k), 0x0040), __byte_perm(code_bits(c, k), code_bits(d, k), 0x0040), 0x5410) & k.keep;
 }
 
 }  // namespace kvad

@@ -10,7 +10,9 @@
 //   t = x + mult * delta;    y = t / sqrt(mean(t^2) + eps) * w        (layer: t less its mean, + b)
 //
 // One pass: a row's entries stay in the registers of its threads from the sum through both reductions (mean square, maximum) to the
-// codes.  Sums, norms and scales are 32-bit; the only rounding to fewer bits is the code itself.
+// codes.  Sums, norms and scales are 32-bit; the only rounding to fewer bits is the code itself.  Bound by memory: 16384 rows of 4096, RMS norm after a sum with
+// bfloat16 results, 113 us (6.5 TB/s; 11 bytes an entry); without the sum 72 (4.7), layer norm 88 (3.8), bfloat16 rows as they are 45 (4.5), where a row's reductions leave
+// its block with nothing in flight (a block that asked for its next row beforehand was slower: 103 for the layer norm; so many registers leave fewer blocks).
 // kvad_int8_read: codes back to numbers.
 //
 // No pointer is __restrict__: what is promised not to change may be read before the wait for the kernel that writes it.
@@ -66,7 +68,7 @@ template <int TPR> __device__ __forceinline__ uint32_t row_max(uint32_t v, float
 
 // TPR threads a row, 4 * V entries a thread at most.  VEC: four entries at a time (every row on a 4-entry boundary), else one.
 template <typename T, int NORM, int TPR, int V, bool VEC>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, V > 4 ? 1 : 1536 / (TPR < 128 ? 128 : TPR))
 int8_rows_kernel(const T* x, int64_t ld_x, const int* rows, const void* delta, int delta_f32, int64_t ld_delta,
                  float mult, float* x_out, int64_t ld_out, const void* weight, const void* bias, int params_f32,
                  int unit_offset, int8_t* codes, int64_t ld_codes, float* scales, int n, int width, float eps) {
@@ -149,13 +151,10 @@ int8_rows_kernel(const T* x, int64_t ld_x, const int* rows, const void* delta, i
       }
     }
   }
-  uint32_t top = 0;                          // largest magnitude, as bits: NaN and infinity are above every finite number
+  float most = 0.f;
 #pragma unroll
-  for (int e = 0; e < 4 * V; ++e) {
-    const uint32_t bits = __float_as_uint(v[e]) & 0x7fffffffu;
-    top = bits > top ? bits : top;
-  }
-  top = row_max<TPR>(top, scratch);
+  for (int e = 0; e < 4 * V; ++e) most = max_abs(most, v[e]);
+  const uint32_t top = row_max<TPR>(__float_as_uint(most), scratch);      // as bits NaN and infinity are above every finite number
   const Scale k = scale_of(top);
   if (t == 0) scales[r] = k.s;
   int8_t* cr = codes + r * ld_codes;
@@ -169,26 +168,46 @@ int8_rows_kernel(const T* x, int64_t ld_x, const int* rows, const void* delta, i
   }
 }
 
+// A thread has READ pieces of 16 bytes of numbers (VEC; else of one number), a block's width apart: whole lines leave together, and all pieces' codes are asked for
+// before the first is worked on.
+constexpr int READ = 4;
+
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
 int8_read_kernel(const int8_t* codes, int64_t ld_codes, const float* scales, T* out, int64_t ld_out, int n, int width) {
   pdl_launch_dependents();
-  const int per_row = VEC ? (width + 15) / 16 : width;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  constexpr int E = VEC ? 16 / sizeof(T) : 1;
+  const uint32_t per_row = (width + E - 1) / E;
+  const int64_t pieces = (int64_t)n * per_row, first = (int64_t)blockIdx.x * (256 * READ) + threadIdx.x;
+  int64_t row[READ];
+  int col[READ];
+  uint2 q[READ];
+  float s[READ];
   pdl_wait();
-  if (i >= (int64_t)n * per_row) return;
-  const int64_t r = i / per_row;
-  const int j = (int)(i - r * per_row) * (VEC ? 16 : 1);
-  const float s = scales[r];
-  if (VEC) {
-    const int4 q = *reinterpret_cast<const int4*>(codes + r * ld_codes + j);
-    const int w[4] = {q.x, q.y, q.z, q.w};
-    T* o = out + r * ld_out + j;
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      store4(o + 4 * k, make_float4((float)(int8_t)w[k] * s, (float)(int8_t)(w[k] >> 8) * s, (float)(int8_t)(w[k] >> 16) * s, (float)(w[k] >> 24) * s));
-  } else {
-    out[r * ld_out + j] = from_f32<T>((float)codes[r * ld_codes + j] * s);
+  for (int u = 0; u < READ; ++u) {
+    const int64_t i = first + u * 256;
+    row[u] = i < pieces ? (pieces >> 32 ? i / per_row : (uint32_t)i / per_row) : -1;
+    col[u] = (int)(i - row[u] * per_row) * E;
+    if (row[u] < 0) continue;
+    const int8_t* c = codes + row[u] * ld_codes + col[u];
+    if (E == 8) q[u] = *reinterpret_cast<const uint2*>(c);
+    else if (E == 4) q[u].x = *reinterpret_cast<const uint32_t*>(c);
+    else q[u].x = (uint8_t)*c;
+    s[u] = scales[row[u]];
+  }
+#pragma unroll
+  for (int u = 0; u < READ; ++u) {
+    if (row[u] < 0) continue;
+    T* o = out + row[u] * ld_out + col[u];
+    if constexpr (VEC) {
+      union { T t[E]; uint4 w; } p;
+#pragma unroll
+      for (int e = 0; e < E; ++e) p.t[e] = from_f32<T>((float)(int8_t)((e < 4 ? q[u].x : q[u].y) >> (8 * (e & 3))) * s[u]);
+      *reinterpret_cast<uint4*>(o) = p.w;
+    } else {
+      *o = from_f32<T>((float)(int8_t)q[u].x * s[u]);
+    }
   }
 }
 
@@ -210,12 +229,18 @@ template <typename T, int NORM, int TPR, int V, bool VEC> cudaError_t go(const C
                      c.params_f32, c.unit_offset, c.codes, c.ld_codes, c.scales, c.n, c.width, c.eps);
 }
 
-// Threads for a row: a warp up to 512 entries, then as many as give each 16 entries, then 32.
+// Threads for a row: a warp up to 512 entries (no barriers), then as many as give each 16 entries, then 32; of the pieces that a thread could have, no more than
+// the width needs.
 template <typename T, int NORM, bool VEC> cudaError_t by_width(const Call& c) {
   if (c.width <= 128) return go<T, NORM, 32, 1, VEC>(c);
+  if (c.width <= 256) return go<T, NORM, 32, 2, VEC>(c);
   if (c.width <= 512) return go<T, NORM, 32, 4, VEC>(c);
+  if (c.width <= 1024) return go<T, NORM, 128, 2, VEC>(c);
+  if (c.width <= 1536) return go<T, NORM, 128, 3, VEC>(c);
   if (c.width <= 2048) return go<T, NORM, 128, 4, VEC>(c);
+  if (c.width <= 256 * 12) return go<T, NORM, 256, 3, VEC>(c);
   if (c.width <= 4096) return go<T, NORM, 256, 4, VEC>(c);
+  if (c.width <= 512 * 12) return go<T, NORM, 512, 3, VEC>(c);
   if (c.width <= 8192) return go<T, NORM, 512, 4, VEC>(c);
   if (c.width <= 16384) return go<T, NORM, 1024, 4, VEC>(c);
   return go<T, NORM, 1024, 8, VEC>(c);
@@ -249,8 +274,9 @@ KVAD_EXPORT int kvad_int8_read(int dtype, const int8_t* codes, int64_t ld_codes,
                                cudaStream_t stream) {
   KVAD_REQUIRE(n > 0 && width > 0, "int8_read: needs rows, got %d of %d entries", n, width);
   const bool f32 = dtype == KVAD_DTYPE_F32;
-  const bool vec = width % 16 == 0 && aligned(codes, ld_codes, 1, 16) && aligned(out, ld_out, f32 ? 4 : 2, 4);
-  const int64_t pieces = (int64_t)n * (vec ? width / 16 : width), blocks = (pieces + 255) / 256;
+  const int e16 = f32 ? 4 : 8;                // entries of 16 bytes
+  const bool vec = width % e16 == 0 && aligned(codes, ld_codes, 1, e16) && aligned(out, ld_out, f32 ? 4 : 2, e16);
+  const int64_t pieces = (int64_t)n * (vec ? width / e16 : width), blocks = (pieces + 256 * READ - 1) / (256 * READ);
   KVAD_REQUIRE(blocks < (1ll << 31), "int8_read: %d rows of %d entries are more than a launch takes", n, width);
   cudaError_t e;
   auto launch = [&](auto kernel, auto* o) { return kvad_launch(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, codes, ld_codes, scales, o, ld_out, n, width); };
