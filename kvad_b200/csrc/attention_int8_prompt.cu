@@ -57,7 +57,7 @@ struct Args {
   const float* ks;
   const int8_t* v;
   const float* vs;
-  int n_seqs, n_heads, kv_heads, window, keep_first, parts, part_pages, skip_copy;
+  int n_seqs, n_heads, kv_heads, window, keep_first, parts, part_pages, skip_copy, sorted;
   float scale_log2;
   int64_t items;                                // rows x heads
   float* scratch;                               // where the pages of a block's rows are dealt out to several blocks: see attention_int8_join.cuh
@@ -147,6 +147,47 @@ __device__ __forceinline__ void tmem_arrived(uint32_t (&x)[PAGE]) {
                : : "memory");
 }
 
+// Sequence and tile (of `tokens` new rows) number `item` in the order of the pages they see, most first; -1 beyond the last.  A warp.  The tiles of a sequence that see
+// P pages or more are its last so many, a number that takes no search: P is found by bisection over the sum of these numbers, then the tile among those of just P.
+__device__ __forceinline__ void longest_first(const Args& a, int item, int tokens, int lane, int& seq, int& tile) {
+  auto tiles_of = [&](int s) { return (a.seq_starts[s + 1] - a.seq_starts[s] + tokens - 1) / tokens; };
+  auto reaching = [&](int s, int p) {                            // the sequence's tiles that see p pages or more
+    const int len = a.kv_lens[s], tiles = tiles_of(s), need = (p - 1) * PAGE - (len - (a.seq_starts[s + 1] - a.seq_starts[s]));
+    return tiles == 0 || len <= (p - 1) * PAGE ? 0 : need < 0 ? tiles : max(1, tiles - need / tokens);      // (tile y reaches position need, counted from its sequence's first new one, if (y + 1) tokens > need)
+  };
+  auto all = [&](int p) {
+    int n = 0;
+    for (int s = lane; s < a.n_seqs; s += 32) n += reaching(s, p);
+    return __reduce_add_sync(0xffffffffu, n);
+  };
+  seq = tile = -1;
+  int lo = 1, hi = a.table_width + 1, above = 0;                 // all(lo) > item >= all(hi) = above
+  if (all(1) <= item) return;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1, n = all(mid);
+    if (n > item) lo = mid;
+    else hi = mid, above = n;
+  }
+  int rank = item - above;
+  for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
+    const int s = s0 + lane, more = s < a.n_seqs ? reaching(s, lo + 1) : 0, n = s < a.n_seqs ? reaching(s, lo) - more : 0;
+    int upto = n;                                                // tiles of just lo pages in this and the lanes before
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    const uint32_t here = __ballot_sync(0xffffffffu, rank < upto);
+    if (here != 0) {
+      const int who = __ffs(here) - 1, before = __shfl_sync(0xffffffffu, upto - n, who), over = __shfl_sync(0xffffffffu, more, who);
+      seq = s0 + who;
+      tile = tiles_of(seq) - 1 - over - (rank - before);
+      return;
+    }
+    rank -= __shfl_sync(0xffffffffu, upto, 31);
+  }
+}
+
 template <int HD>
 __global__ void __launch_bounds__(THREADS, 1)
 attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ Args a) {
@@ -174,10 +215,20 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   const int group = a.n_heads / a.kv_heads, tok = ROWS / group;  // tokens of a slot
-  const int columns = a.n_seqs * a.kv_heads, from_end = blockIdx.x / columns, column = blockIdx.x - from_end * columns;
-  const int s = column / a.kv_heads, kvh = column - s * a.kv_heads;
+  const int item = blockIdx.x / a.kv_heads, kvh = blockIdx.x - item * a.kv_heads;
+  __shared__ int chosen[2];
+  if (a.sorted) {
+    if (warp == 0) {
+      int ts, tt;
+      longest_first(a, item, 2 * tok, lane, ts, tt);
+      if (lane == 0) chosen[0] = ts, chosen[1] = tt;
+    }
+    __syncthreads();
+    if (chosen[0] < 0) return;
+  }
+  const int from_end = item / a.n_seqs, s = a.sorted ? chosen[0] : item - from_end * a.n_seqs;
   const int row0 = a.seq_starts[s], n_new = a.seq_starts[s + 1] - row0;
-  const int tile = (n_new + 2 * tok - 1) / (2 * tok) - 1 - from_end;      // the last rows, which see the most, first
+  const int tile = a.sorted ? chosen[1] : (n_new + 2 * tok - 1) / (2 * tok) - 1 - from_end;
   if (tile < 0) return;
   const int kv_len = a.kv_lens[s];
   const int* pages = a.table + (int64_t)s * a.table_width;
@@ -526,8 +577,18 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
   }
 }
 
+int sm_count() {
+  static int n = 0;
+  if (n == 0) {
+    int dev = 0, v = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && v > 0) n = v;
+    else n = 148;
+  }
+  return n;
+}
+
 template <int HD>
-int launch(const void* q, int64_t ld_q, int n_rows, const Args& a, int max_new, cudaStream_t stream) {
+int launch(const void* q, int64_t ld_q, int n_rows, Args a, int max_new, cudaStream_t stream) {
   using L = Layout<HD>;
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) KVAD_FAIL(KVAD_ERR_CUDA, "attention_int8_prompt: the driver does not offer cuTensorMapEncodeTiled");
@@ -551,6 +612,9 @@ int launch(const void* q, int64_t ld_q, int n_rows, const Args& a, int max_new, 
   }
   const int64_t blocks = (int64_t)((max_new + 2 * tok - 1) / (2 * tok)) * a.n_seqs * a.kv_heads;
   KVAD_REQUIRE(blocks < (1ll << 31) && a.parts <= 65535, "attention_int8_prompt: more rows and heads than a launch takes");
+  // more blocks than SMs: the longest first, so that none of them starts late (prompts in pieces of 512 behind 7680, 4096, 6002 and 1024 positions, 32 heads of 128
+  // on 8: 227 us against 263 with every sequence's last rows first).  (A warp looks the order up in every block; beyond so many sequences that takes microseconds.)
+  a.sorted = blocks * a.parts > sm_count() && a.n_seqs <= 256;
   cudaError_t e = kvad_launch(kernel, dim3((unsigned)blocks, a.parts), dim3(THREADS), L::SMEM, stream, map, a);
   if (e == cudaSuccess && a.parts > 1) e = join_blocks<__nv_bfloat16>(a.scratch, a.out, a.ld_out, n_rows, a.n_heads, HD, a.parts, stream);
   if (e != cudaSuccess) KVAD_FAIL(KVAD_ERR_CUDA, "attention_int8_prompt: launch failed: %s", cudaGetErrorString(e));
@@ -575,7 +639,7 @@ KVAD_EXPORT int kvad_attention_int8_prompt(const void* q, int64_t ld_q, void* ou
   KVAD_REQUIRE(window >= 0 && keep_first >= 0, "attention_int8_prompt: a window and kept first positions cannot be negative");
   KVAD_REQUIRE(parts >= 1 && (parts == 1 || (part_pages > 0 && scratch != nullptr)), "attention_int8_prompt: no way to deal out pages: %d, %d", parts, part_pages);
   Args a{reinterpret_cast<__nv_bfloat16*>(out), ld_o, seq_starts, kv_lens, table, table_width, k_pages, k_scales, v_pages, v_scales,
-         n_seqs, n_heads, kv_heads, window, window > 0 ? keep_first : 0, parts, part_pages, g_skip_copy ? 1 : 0, scale * LOG2E, (int64_t)n_rows * n_heads, reinterpret_cast<float*>(scratch)};
+         n_seqs, n_heads, kv_heads, window, window > 0 ? keep_first : 0, parts, part_pages, g_skip_copy ? 1 : 0, 0, scale * LOG2E, (int64_t)n_rows * n_heads, reinterpret_cast<float*>(scratch)};
   g_skip_copy = false;
   switch (hd) {
     case 16: return launch<16>(q, ld_q, n_rows, a, max_new, stream);
