@@ -65,16 +65,18 @@ struct Args {
 
 template <int HD> struct Layout {
   static constexpr int BLOCKS = (HD + 63) / 64;                  // of 64 entries: 128 bytes
-  static constexpr int RING = HD > 64 ? 6 : 8, RAW = 6;         // pages of keys or values in half precision, and as they came
+  // Pages of keys, and as many of values, in half precision and as they came.  (Rings of their own: who waits on a barrier's phase has to have seen the one before,
+  // or takes a barrier that is still in that one for one that has passed the next.)
+  static constexpr int RING = HD > 64 ? 3 : 4, RAW = 3;
   static constexpr uint32_t Q_BYTES = BLOCKS * Q_BLOCK, KV_BYTES = BLOCKS * PAGE_BLOCK;
   static constexpr uint32_t CODES = PAGE * HD, RAW_BYTES = CODES + 2 * PAGE * 4;
   static constexpr uint32_t SET = 16 + PAGE * 4;                 // what softmax threads need of a page, and marks of its keys
-  static constexpr uint32_t OFF_KV = 2 * Q_BYTES, OFF_RAW = OFF_KV + RING * KV_BYTES, OFF_SC = OFF_RAW + RAW * RAW_BYTES;
+  static constexpr uint32_t OFF_KV = 2 * Q_BYTES, OFF_RAW = OFF_KV + 2 * RING * KV_BYTES, OFF_SC = OFF_RAW + 2 * RAW * RAW_BYTES;
   static constexpr uint32_t OFF_BAR = OFF_SC + SETS * SET;
-  static constexpr int BARS = 1 + 2 * RING + 2 * RAW + 2 * 7;
+  static constexpr int BARS = 1 + 4 * RING + 4 * RAW + 2 * 7;
   static constexpr size_t SMEM = OFF_BAR + BARS * 8 + 16 + 1024;
   static constexpr uint32_t TM_O = 256;                          // S (and P) of slot t at t * 128 + 64 in turn, its output at TM_O + t * 128
-  static_assert(SETS >= RING / 2 + 2, "a page's set is read until the products of the page before are done");
+  static_assert(SETS >= RING + 2, "a page's set is read until the products of the page before are done");
   static_assert(SMEM <= 227 * 1024, "an SM's shared memory");
 };
 
@@ -200,11 +202,11 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
   uint8_t* raw_tiles = smem + L::OFF_RAW;
   uint8_t* sets = smem + L::OFF_SC;                              // [SETS]: of a page {2^(b - 8), c, 2^-c, whether a value's scale is not finite}, then a mark a key
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
-  uint64_t* kv_full = q_full + 1;                                // [RING] a page's keys or values are half precision
-  uint64_t* kv_empty = kv_full + RING;                           // [RING] both slots' products have read them
-  uint64_t* raw_full = kv_empty + RING;                          // [RAW] a page's codes and scales have come
-  uint64_t* raw_empty = raw_full + RAW;                          // [RAW] they have been turned
-  uint64_t* s_full = raw_empty + RAW;                            // [slot][2] S is in tensor memory
+  uint64_t* kv_full = q_full + 1;                                // [keys, values][RING] a page is half precision
+  uint64_t* kv_empty = kv_full + 2 * RING;                         // [keys, values][RING] both slots' products have read them
+  uint64_t* raw_full = kv_empty + 2 * RING;                         // [keys, values][RAW] a page's codes and scales have come
+  uint64_t* raw_empty = raw_full + 2 * RAW;                         // [keys, values][RAW] they have been turned
+  uint64_t* s_full = raw_empty + 2 * RAW;                         // [slot][2] S is in tensor memory
   uint64_t* p_full = s_full + 4;                                 // [slot][2] P is (and S has been read)
   uint64_t* t_full = p_full + 4;                                 // [slot][2] P V of a page has been added (two in turn: a wait for the latest must not take one before for it)
   uint64_t* q_ready = t_full + 4;                                // [slot] its queries are half precision
@@ -254,8 +256,8 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
   if (threadIdx.x == 0) {
     prefetch_tensormap(&map_q);
     mbar_init(q_full, 1);
-    for (int i = 0; i < RING; ++i) { mbar_init(&kv_full[i], 128); mbar_init(&kv_empty[i], 2); }
-    for (int i = 0; i < RAW; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 4); }
+    for (int i = 0; i < 2 * RING; ++i) { mbar_init(&kv_full[i], 128); mbar_init(&kv_empty[i], 2); }
+    for (int i = 0; i < 2 * RAW; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 4); }
     for (int i = 0; i < 4; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); mbar_init(&t_full[i], 1); }
     for (int i = 0; i < 2; ++i) mbar_init(&q_ready[i], 128);
     failed = 0;
@@ -278,20 +280,18 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
         for (int t = 0; t < (n_tok1 > 0 ? 2 : 1); ++t)
           for (int b = 0; b < L::BLOCKS; ++b)
             tma_load_3d(q_tiles + t * L::Q_BYTES + b * Q_BLOCK, &map_q, q_full, b * 64, kvh * group, row0 + tok0 + t * tok);
-        int r = 0;
-        uint32_t phase = 1;                                      // (the first round finds the ring empty)
         // keys of page 0, then keys of the next page and values of this one in turn: the order of use
         for (int n = 0; n < 2 * units && ok; ++n) {
           const bool values = n == 2 * units - 1 || (n > 0 && (n & 1) == 0);
           const int u = n == 2 * units - 1 ? units - 1 : values ? n / 2 - 1 : (n + 1) / 2;
           const int64_t cell = ((int64_t)pages[page_of(u)] * a.kv_heads + kvh) * PAGE;
-          if (!mbar_wait(&raw_empty[r], phase)) { ok = false; break; }
+          const int r = (values ? RAW : 0) + u % RAW;
+          if (!mbar_wait(&raw_empty[r], ((u / RAW) & 1) ^ 1)) { ok = false; break; }      // (the first round finds the ring empty)
           uint8_t* dst = raw_tiles + r * L::RAW_BYTES;
           mbar_expect_tx(&raw_full[r], L::CODES + (values ? 1 : 2) * PAGE * 4);
           if (!(a.skip_copy && n == 0)) bulk_copy(dst, (values ? a.v : a.k) + cell * HD, L::CODES, &raw_full[r]);
           bulk_copy(dst + L::CODES, a.vs + cell, PAGE * 4, &raw_full[r]);        // (values' scales with the keys too: scores want the pages' exponents)
           if (!values) bulk_copy(dst + L::CODES + PAGE * 4, a.ks + cell, PAGE * 4, &raw_full[r]);
-          if (++r == RAW) r = 0, phase ^= 1;
         }
       }
     } else if (warp < 3) {
@@ -302,47 +302,46 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
       const uint64_t q_desc = sw128_desc(smem_u32(q_tiles + t * L::Q_BYTES)), k_desc = sw128_desc(smem_u32(kv_tiles));
       const uint64_t v_desc = sw128_mn_desc(smem_u32(kv_tiles));
       const uint32_t tm_s = tmem + t * 128, tm_o = tmem + L::TM_O + t * 128;
-      int r = 0;
-      uint32_t phase = 0;
-      auto next = [&] { if (++r == RING) r = 0, phase ^= 1; };
+      int rk = 0, rv = 0;                                        // places of the next keys and values
+      uint32_t phase_k = 0, phase_v = 0;
       if (mine > 0) ok = mbar_wait(&q_ready[t], 0);
       // keys of page i + 1, then values of page i: from page -1 on, which has no values, to the last, which has no next
       for (int i = -1; i < units && ok; ++i) {
         if (i + 1 < units) {
           if (i + 1 < mine && i > 0 && !mbar_wait(&t_full[t * 2 + ((i - 1) & 1)], ((i - 1) >> 1) & 1)) { ok = false; break; }      // P V of page i - 1 has read what S goes over
-          if (!mbar_wait(&kv_full[r], phase)) { ok = false; break; }
+          if (!mbar_wait(&kv_full[rk], phase_k)) { ok = false; break; }
           if (i + 1 < mine) {
             tc_fence_after();
             if (one) {
-              const uint64_t at = k_desc + (uint32_t)r * (L::KV_BYTES >> 4);
+              const uint64_t at = k_desc + (uint32_t)rk * (L::KV_BYTES >> 4);
 #pragma unroll
               for (int k = 0; k < HD / 16; ++k)
                 umma(tm_s + ((i + 1) & 1) * PAGE, q_desc + (uint64_t)((k / 4) * (Q_BLOCK >> 4) + (k % 4) * 2), at + (uint64_t)((k / 4) * (PAGE_BLOCK >> 4) + (k % 4) * 2),
                      idesc_s, k > 0 ? 1u : 0u);
               umma_commit(&s_full[t * 2 + ((i + 1) & 1)]);
-              umma_commit(&kv_empty[r]);
+              umma_commit(&kv_empty[rk]);
             }
           } else if (lane == 0) {
-            mbar_arrive_one(&kv_empty[r]);                       // (the other slot walks on: what comes goes back unread)
+            mbar_arrive_one(&kv_empty[rk]);                       // (the other slot walks on: what comes goes back unread)
           }
-          next();
+          if (++rk == RING) rk = 0, phase_k ^= 1;
         }
         if (i >= 0) {
           if (i < mine && !mbar_wait(&p_full[t * 2 + (i & 1)], (i >> 1) & 1)) { ok = false; break; }
-          if (!mbar_wait(&kv_full[r], phase)) { ok = false; break; }
+          if (!mbar_wait(&kv_full[RING + rv], phase_v)) { ok = false; break; }
           if (i < mine) {
             tc_fence_after();
             if (one) {
-              const uint64_t at = v_desc + (uint32_t)r * (L::KV_BYTES >> 4);
+              const uint64_t at = v_desc + (uint32_t)(RING + rv) * (L::KV_BYTES >> 4);
 #pragma unroll
               for (int k = 0; k < PAGE / 16; ++k) umma_ta(tm_o, tm_s + (i & 1) * PAGE + k * 8, at + (uint64_t)(k * (2048 >> 4)), idesc_t, (i > 0 || k > 0) ? 1u : 0u);
               umma_commit(&t_full[t * 2 + (i & 1)]);
-              umma_commit(&kv_empty[r]);
+              umma_commit(&kv_empty[RING + rv]);
             }
           } else if (lane == 0) {
-            mbar_arrive_one(&kv_empty[r]);
+            mbar_arrive_one(&kv_empty[RING + rv]);
           }
-          next();
+          if (++rv == RING) rv = 0, phase_v ^= 1;
         }
       }
     }
@@ -353,9 +352,8 @@ attention_int8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __
     int exponent = -64;                                          // of the values of the page (a page of zeros takes that of the one before)
     auto turn = [&](auto which, int u) {                         // keys or values of page u
       constexpr bool VALUES = decltype(which)::value;
-      const int n = VALUES ? (u == units - 1 ? 2 * units - 1 : 2 * u + 2) : max(0, 2 * u - 1);      // its place in the order of use
-      const int r = n % RING, raw = n % RAW;
-      if (!mbar_wait(&kv_empty[r], ((n / RING) & 1) ^ 1) || !mbar_wait(&raw_full[raw], (n / RAW) & 1)) { ok = false; return; }
+      const int r = (VALUES ? RING : 0) + u % RING, raw = (VALUES ? RAW : 0) + u % RAW;
+      if (!mbar_wait(&kv_empty[r], ((u / RING) & 1) ^ 1) || !mbar_wait(&raw_full[raw], (u / RAW) & 1)) { ok = false; return; }
       uint8_t* dst = kv_tiles + r * L::KV_BYTES;
       const uint8_t* src = raw_tiles + raw * L::RAW_BYTES;
       const float* vs = reinterpret_cast<const float*>(src + L::CODES);

@@ -440,7 +440,7 @@ class Ops:
         return (_switch_epoch, self.tensor_core_linear, self.tensor_core_prefill, self.fast_decode,
                 self.rows_linear_max, self.qkv_sums, self.SUMS_MIN_K, self.tiled_prompt, self.split_linear, self.pieces_linear, self.scored_prompt, self.scored_wide, self.chunked_recurrences,
                 self.SPLIT_MIN_ROWS, self.PIECES_MIN_ROWS, self.PIECES_MIN_K, self.PIECES_ONE_TILE, self.PIECES_WORK_BYTES, self.SCORED_PROMPT_MIN_NEW, self.SHORT_PROMPT_KEYS, self.SHORT_PROMPT_MAX, self.CHUNK_MIN_ROWS, self.CHUNK_SHORT_ROWS, self.CHUNK_WORK_BYTES,
-                self.ROWS_LINEAR_MAX_OUT, self.ROWS_BLOCKS_MAX, self.HEADS_LINEAR_MAX_ROWS)
+                self.ROWS_LINEAR_MAX_OUT, self.ROWS_BLOCKS_MAX, self.HEADS_LINEAR_MAX_ROWS, self.INT8_PROMPT_HEAD_SIZES)
 
     def begin_step(self) -> None:
         """Called once before a step's first kernel (inside the capture, if the step is being captured)."""
@@ -2192,14 +2192,23 @@ def scored_wide_wait_timeouts() -> int:
     return n
 
 
+def _timeouts(library: str) -> int:
+    h = lib(library)
+    n = getattr(h, f"kvad_{library}_status")()
+    if n < 0:
+        raise KernelError(f"{library}: the number of waits that ran out cannot be read")
+    return n
+
+
 def linear_int8_wait_timeouts() -> int:
     """How many bounded waits of the products of 8-bit rows have run out in this process (0 unless something is wrong).  Synchronises the device."""
-    return int(lib("linear_int8").kvad_linear_int8_status())
+    return _timeouts("linear_int8")
 
 
 def attention_int8_wait_timeouts() -> int:
-    """How many bounded waits of the prompt attention over 8-bit caches have run out in this process (0 unless something is wrong).  Synchronises the device."""
-    return int(lib("attention_int8_prompt").kvad_attention_int8_prompt_status())
+    """How many bounded waits of the attention over 8-bit caches, of prompts and of single tokens, have run out in this process (0 unless something is wrong).
+    Synchronises the device."""
+    return _timeouts("attention_int8_prompt") + _timeouts("attention_int8")
 
 
 def scored_prompt_wait_timeouts() -> int:
@@ -2212,7 +2221,7 @@ def scored_prompt_wait_timeouts() -> int:
 
 
 def wait_test_hooks(library: str, wait_limit: int = 0, skip_copy: bool = False) -> None:
-    """Tests of the bounded waits of "linear_pieces", "attention_scored_prompt" and "attention_scored_wide": `wait_limit` polls before a wait gives up
+    """Tests of the bounded waits of "linear_pieces", "attention_scored_prompt", "attention_scored_wide", "linear_int8", "attention_int8" and "attention_int8_prompt": `wait_limit` polls before a wait gives up
     (0: the library's own limit), and a copy that the next launch's blocks leave out."""
     h = lib(library)
     if getattr(h, f"kvad_{library}_test_hooks")(int(wait_limit), int(bool(skip_copy))) != 0:
