@@ -7,8 +7,8 @@
 //
 // so a position takes head size + 4 bytes a head, where bfloat16 takes 2 * head size.
 //
-// A group of lanes (a power of two, head size / 8 at least) has one row, and of it one head's keys or values, or four heads' where there are many rows: a lane
-// brings eight entries, the group's maximum is a few shuffles, and the codes leave as eight bytes a lane.  Where a row goes is looked up once for the four heads
+// A group of lanes (a power of two, head size / 8 at least) has one row, and of it one head's keys or values, or several heads' where there are many rows: a lane
+// brings eight entries, the group's maximum is a few shuffles, and the codes leave as eight bytes a lane.  Where a row goes is looked up once for these heads
 // (a chain of two trips to memory), and all their entries are asked for before the first is worked on.  Bound by memory, entry + 1 bytes
 // a code: 26289 bfloat16 rows of 8 heads of 128 are stored in 41 us (3.9 TB/s; four rows of one head a group: 79) and read in 30 (5.5 TB/s).
 //
@@ -23,28 +23,30 @@ KVAD_DEFINE_LAST_ERROR()
 
 namespace {
 
-// Eight consecutive entries as floats; `vec`: on a boundary of 16 bytes.
-__device__ __forceinline__ void load8(const float* p, bool vec, float* v) {
+// Eight consecutive entries as they lie, and as floats; `vec`: on a boundary of 16 bytes.
+template <typename T> struct Eight { uint4 w[sizeof(T) / 2]; };
+template <typename T> __device__ __forceinline__ void load8(const T* p, bool vec, Eight<T>& x) {
   if (vec) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = p[i];
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) x.w[i] = reinterpret_cast<const uint4*>(p)[i];
+  } else {
+    T* t = reinterpret_cast<T*>(&x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = p[i];
   }
 }
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, bool vec, float* v) {
-  if (vec) {
-    const uint4 q = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+__device__ __forceinline__ void numbers(const Eight<float>& x, float* v) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = __uint_as_float(w[i] << 16);
-      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-  } else {
+  for (int i = 0; i < 2; ++i) {
+    v[4 * i] = __uint_as_float(x.w[i].x); v[4 * i + 1] = __uint_as_float(x.w[i].y); v[4 * i + 2] = __uint_as_float(x.w[i].z); v[4 * i + 3] = __uint_as_float(x.w[i].w);
+  }
+}
+__device__ __forceinline__ void numbers(const Eight<__nv_bfloat16>& x, float* v) {
+  const uint32_t w[4] = {x.w[0].x, x.w[0].y, x.w[0].z, x.w[0].w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __bfloat162float(p[i]);
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
   }
 }
 __device__ __forceinline__ void store8(float* p, bool vec, const float* v) {
@@ -85,7 +87,7 @@ struct Pages {
 
 // blockIdx.y: so many heads, blockIdx.z: their keys (0) or values (1).  Addresses step from head to head: worked out a head, they are half of the instructions.
 template <typename T, int LANES, int R>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 4)
 int8_store_kernel(const T* k_src, const T* v_src, int64_t ld_src, int vec, const Pages p, int8_t* k_pages,
                   float* k_scales, int8_t* v_pages, float* v_scales, int n) {
   pdl_launch_dependents();
@@ -93,23 +95,24 @@ int8_store_kernel(const T* k_src, const T* v_src, int64_t ld_src, int vec, const
   const int heads = row < n && lane * 8 < p.hd ? min(R, p.heads - head) : 0;
   const T* src = (blockIdx.z ? v_src : k_src) + row * ld_src + (head * p.hd + lane * 8);
   pdl_wait();
-  float v[R][8] = {};
+  Eight<T> x[R] = {};
 #pragma unroll
   for (int i = 0; i < R; ++i)
-    if (i < heads) load8(src + i * p.hd, vec, v[i]);
+    if (i < heads) load8(src + i * p.hd, vec, x[i]);
   const int64_t cell = heads > 0 ? p.cell(row, head) : 0;
   int8_t* to = (blockIdx.z ? v_pages : k_pages) + cell * p.hd + lane * 8;
   float* scale = (blockIdx.z ? v_scales : k_scales) + cell;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    float most = 0.f;
+    float v[8], most = 0.f;
+    numbers(x[i], v);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) most = max_abs(most, v[i][e]);
+    for (int e = 0; e < 8; ++e) most = max_abs(most, v[e]);
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) most = max_abs(most, __shfl_xor_sync(0xffffffffu, most, o));
     if (i >= heads) continue;
     const Scale k = scale_of(__float_as_uint(most));
-    *reinterpret_cast<uint2*>(to) = make_uint2(codes_of(v[i][0], v[i][1], v[i][2], v[i][3], k), codes_of(v[i][4], v[i][5], v[i][6], v[i][7], k));
+    *reinterpret_cast<uint2*>(to) = make_uint2(codes_of(v[0], v[1], v[2], v[3], k), codes_of(v[4], v[5], v[6], v[7], k));
     if (lane == 0) *scale = k.s;
     to += p.page * p.hd;
     scale += p.page;
@@ -164,7 +167,7 @@ int check(const char* what, int n, int heads, int hd, int page, int table_width,
   return KVAD_OK;
 }
 
-constexpr int MANY = 512;        // rows from which on a group of lanes takes four heads of its row
+constexpr int MANY = 512;        // rows from which on a group of lanes takes several heads of its row
 
 Pages pages(const int* row_seq, const int* row_pos, const int* table, int width, int heads, int hd, int page) {
   int shift = -1;
@@ -193,7 +196,8 @@ KVAD_EXPORT int kvad_kv_store_int8(int dtype, const void* k_src, const void* v_s
     };
     auto go = [&](auto* k, auto* v) {
       using T = std::remove_cv_t<std::remove_pointer_t<decltype(k)>>;
-      return n >= MANY ? launch(int8_store_kernel<T, L, 4>, 4, k, v) : launch(int8_store_kernel<T, L, 1>, 1, k, v);
+      constexpr int R = sizeof(T) == 2 ? 8 : 4;              // (128 bytes a lane)
+      return n >= MANY ? launch(int8_store_kernel<T, L, R>, R, k, v) : launch(int8_store_kernel<T, L, 1>, 1, k, v);
     };
     return dtype == KVAD_DTYPE_F32 ? go((const float*)k_src, (const float*)v_src) : go((const __nv_bfloat16*)k_src, (const __nv_bfloat16*)v_src);
   });

@@ -379,9 +379,10 @@ def _need_cuda(*tensors) -> None:
 
 def _rows_view(t: torch.Tensor, what: str) -> int:
     """Leading dimension of a 2-D tensor whose rows are contiguous."""
-    if t.dim() != 2 or t.stride(1) != 1:
-        raise KernelError(f"{what}: needs a 2-D tensor with contiguous rows, got shape {tuple(t.shape)} strides {t.stride()}")
-    return t.stride(0)
+    strides = t.stride()                # (one call: each costs a tenth of a microsecond or two, of a call's ten)
+    if len(strides) != 2 or strides[1] != 1:
+        raise KernelError(f"{what}: needs a 2-D tensor with contiguous rows, got shape {tuple(t.shape)} strides {strides}")
+    return strides[0]
 
 
 @functools.lru_cache(maxsize=256)
@@ -1802,11 +1803,11 @@ class Ops:
 
     @staticmethod
     def _int8_rows_check(what: str, codes, scales, n: int, width: int) -> int:
-        if codes.dtype != torch.int8 or codes.shape != (n, width):
+        if codes.dtype is not torch.int8 or codes.shape != (n, width):
             raise KernelError(f"{what}: codes must be int8 of shape [{n}, {width}]")
-        if scales.dtype != torch.float32 or scales.numel() != n or not scales.is_contiguous():
+        if scales.dtype is not torch.float32 or scales.numel() != n or not scales.is_contiguous():
             raise KernelError(f"{what}: scales must be contiguous float32, one per row")
-        return _rows_view(codes, f"{what} codes")
+        return _rows_view(codes, "8-bit codes")
 
     def int8_rows(self, x, codes, scales) -> None:
         """Rows of activations or weights (float32 or bfloat16) as 8-bit codes and a scale a row."""
@@ -1820,33 +1821,39 @@ class Ops:
 
     def _norm_int8(self, what: str, norm: int, x, weight, bias, eps: float, codes, scales, unit_offset: bool, rows, delta, mult: float, x_out) -> None:
         _need_cuda(x, weight, bias, codes, scales, rows, delta, x_out)
-        ld_x = _rows_view(x, f"{what} input")
-        width = x.shape[1]
-        n = x.shape[0] if rows is None else rows.numel()
-        if x.dtype != torch.float32:
+        f32, bf16 = torch.float32, torch.bfloat16
+        ld_x = _rows_view(x, "stream of a norm to 8 bits")
+        shape = x.shape
+        n, width = shape
+        if rows is not None:
+            n = rows.numel()
+        if x.dtype is not f32:
             raise KernelError(f"{what}: input must be the float32 residual stream")
         ld_c = self._int8_rows_check(what, codes, scales, n, width)
         p_f32 = 0
         for p in (weight, bias):
             if p is not None:
-                if p.numel() != width or p.dtype not in (torch.float32, torch.bfloat16) or not p.is_contiguous():
+                dtype = p.dtype
+                if p.numel() != width or (dtype is not f32 and dtype is not bf16) or not p.is_contiguous():
                     raise KernelError(f"{what}: weight and bias must have the row's width, float32 or bfloat16")
-                p_f32 = 1 if p.dtype == torch.float32 else 0
+                p_f32 = 1 if dtype is f32 else 0
         if weight is not None and bias is not None and weight.dtype != bias.dtype:
             raise KernelError(f"{what}: weight and bias must have one dtype")
         if rows is not None and (rows.dtype != torch.int32 or not rows.is_contiguous() or delta is not None or x_out is not None):
             raise KernelError(f"{what}: a row list is contiguous int32, and goes without a sum")
         ld_d = ld_o = d_f32 = 0
         if delta is not None:
-            ld_d = _rows_view(delta, f"{what} sum")
-            if delta.shape != x.shape or delta.dtype not in (torch.float32, torch.bfloat16):
+            ld_d, dtype = _rows_view(delta, "sum of a norm to 8 bits"), delta.dtype
+            if delta.shape != shape or (dtype is not f32 and dtype is not bf16):
                 raise KernelError(f"{what}: what is added must have the stream's shape, float32 or bfloat16")
-            d_f32 = 1 if delta.dtype == torch.float32 else 0
+            d_f32 = 1 if dtype is f32 else 0
             if x_out is None:
                 x_out = x
-        if x_out is not None:
-            ld_o = _rows_view(x_out, f"{what} stream")
-            if x_out.shape != x.shape or x_out.dtype != torch.float32:
+        if x_out is x:
+            ld_o = ld_x
+        elif x_out is not None:
+            ld_o = _rows_view(x_out, "stream after a sum")
+            if x_out.shape != shape or x_out.dtype is not f32:
                 raise KernelError(f"{what}: the stream's output must be float32 of its shape")
         h = lib("int8_rows")
         _check(h.kvad_int8_rows(F32, norm, x.data_ptr(), ld_x, _ptr(rows), _ptr(delta), d_f32, ld_d, float(mult), _ptr(x_out), ld_o, _ptr(weight), _ptr(bias),
@@ -1879,16 +1886,17 @@ class Ops:
         epi = EPILOGUES[epilogue]
         lda, ldo = _rows_view(a, "linear_int8 input"), _rows_view(out, "linear_int8 output")
         m, k = a.shape
-        n = weight.shape[0]
-        if weight.dim() != 2 or weight.shape[1] != k or not weight.is_contiguous():
-            raise KernelError(f"linear_int8: weight {tuple(weight.shape)} does not take inputs of width {k}")
-        if a.dtype != torch.int8 or weight.dtype != torch.int8:
+        w_shape, i8, f32 = weight.shape, torch.int8, torch.float32
+        if len(w_shape) != 2 or w_shape[1] != k or not weight.is_contiguous():
+            raise KernelError(f"linear_int8: weight {tuple(w_shape)} does not take inputs of width {k}")
+        n = w_shape[0]
+        if a.dtype is not i8 or weight.dtype is not i8:
             raise KernelError("linear_int8: input and weight must be int8")
-        if (a_scales.dtype != torch.float32 or a_scales.numel() != m or not a_scales.is_contiguous() or w_scales.dtype != torch.float32
+        if (a_scales.dtype is not f32 or a_scales.numel() != m or not a_scales.is_contiguous() or w_scales.dtype is not f32
                 or w_scales.numel() != n or not w_scales.is_contiguous()):
             raise KernelError("linear_int8: scales must be contiguous float32, one per row and one per output")
-        want_out = torch.float32 if epi >= 3 else self.dtype
-        if out.dtype != want_out or out.shape[0] != m or out.shape[1] != n:
+        want_out = f32 if epi >= 3 else self.dtype
+        if out.dtype is not want_out or out.shape != (m, n):
             raise KernelError(f"linear_int8: output must be {want_out} of shape [{m}, {n}]")
         bias_f32 = 0
         if bias is not None:
@@ -1901,14 +1909,15 @@ class Ops:
 
     @staticmethod
     def _int8_pages(what: str, k_pages, k_scales, v_pages, v_scales) -> tuple:
-        if k_pages.dim() != 4 or k_pages.dtype != torch.int8 or v_pages.dtype != torch.int8 or v_pages.shape != k_pages.shape \
-                or not k_pages.is_contiguous() or not v_pages.is_contiguous():
+        shape, i8, f32 = k_pages.shape, torch.int8, torch.float32
+        if len(shape) != 4 or k_pages.dtype is not i8 or v_pages.dtype is not i8 or v_pages.shape != shape or not k_pages.is_contiguous() or not v_pages.is_contiguous():
             raise KernelError(f"{what}: pages must be contiguous int8 [pages, kv heads, page size, head size], keys and values alike")
-        cells = k_pages.shape[:3]
-        if k_scales.dtype != torch.float32 or v_scales.dtype != torch.float32 or k_scales.shape != cells or v_scales.shape != cells \
-                or not k_scales.is_contiguous() or not v_scales.is_contiguous():
+        pages, n_kv, page, hd = shape
+        cells = (pages, n_kv, page)
+        if k_scales.dtype is not f32 or v_scales.dtype is not f32 or k_scales.shape != cells or v_scales.shape != cells or not k_scales.is_contiguous() \
+                or not v_scales.is_contiguous():
             raise KernelError(f"{what}: scales must be contiguous float32 [pages, kv heads, page size]")
-        return k_pages.shape
+        return pages, n_kv, page, hd
 
     def kv_store_int8(self, k_src, v_src, row_seq, row_pos, page_table, k_pages, k_scales, v_pages, v_scales) -> None:
         """Writes the rows' keys and values (views `[rows, kv_heads * head_dim]` of one buffer) into their sequences' pages as 8-bit codes, with a
@@ -1916,34 +1925,37 @@ class Ops:
         _need_cuda(k_src, v_src, row_seq, row_pos, page_table, k_pages, k_scales, v_pages, v_scales)
         ld = _rows_view(k_src, "new keys")
         _, n_kv, page, hd = self._int8_pages("kv_store_int8", k_pages, k_scales, v_pages, v_scales)
-        n = k_src.shape[0]
-        if (_rows_view(v_src, "new values") != ld or k_src.shape != (n, n_kv * hd) or v_src.shape != k_src.shape or k_src.dtype != self.dtype
-                or v_src.dtype != self.dtype):
-            raise KernelError(f"kv_store_int8: keys and values must be {self.dtype} views [rows, {n_kv} x {hd}] of one buffer")
-        self._rows_of_pages("kv_store_int8", n, row_seq, row_pos, page_table)
+        shape, dtype = k_src.shape, self.dtype
+        n, width = shape
+        if _rows_view(v_src, "new values") != ld or width != n_kv * hd or v_src.shape != shape or k_src.dtype is not dtype or v_src.dtype is not dtype:
+            raise KernelError(f"kv_store_int8: keys and values must be {dtype} views [rows, {n_kv} x {hd}] of one buffer")
+        reach = self._rows_of_pages("kv_store_int8", n, row_seq, row_pos, page_table)
         h = lib("int8_cache")
         _check(h.kvad_kv_store_int8(self.code, k_src.data_ptr(), v_src.data_ptr(), ld, row_seq.data_ptr(), row_pos.data_ptr(), page_table.data_ptr(),
-                                    page_table.shape[1], k_pages.data_ptr(), k_scales.data_ptr(), v_pages.data_ptr(), v_scales.data_ptr(), n, n_kv, hd, page,
+                                    reach, k_pages.data_ptr(), k_scales.data_ptr(), v_pages.data_ptr(), v_scales.data_ptr(), n, n_kv, hd, page,
                                     _stream()), h)
 
     @staticmethod
-    def _rows_of_pages(what: str, n: int, row_seq, row_pos, page_table) -> None:
-        if (row_seq.dtype != torch.int32 or row_pos.dtype != torch.int32 or row_seq.numel() < n or row_pos.numel() < n or page_table.dtype != torch.int32
-                or page_table.dim() != 2 or not page_table.is_contiguous()):
+    def _rows_of_pages(what: str, n: int, row_seq, row_pos, page_table) -> int:
+        i32, shape = torch.int32, page_table.shape
+        if (row_seq.dtype is not i32 or row_pos.dtype is not i32 or row_seq.numel() < n or row_pos.numel() < n or page_table.dtype is not i32
+                or len(shape) != 2 or not page_table.is_contiguous()):
             raise KernelError(f"{what}: the rows' sequences and positions are int32, one per row, and the page table a contiguous int32 matrix")
+        return shape[1]
 
     def kv_read_int8(self, row_seq, row_pos, page_table, k_pages, k_scales, v_pages, v_scales, k_out, v_out) -> None:
         """What the cache holds for the rows: k_out, v_out `[rows, kv_heads * head_dim]` = codes * scale of each row's sequence and position."""
         _need_cuda(row_seq, row_pos, page_table, k_pages, k_scales, v_pages, v_scales, k_out, v_out)
         _, n_kv, page, hd = self._int8_pages("kv_read_int8", k_pages, k_scales, v_pages, v_scales)
-        n = k_out.shape[0]
         ld_k, ld_v = _rows_view(k_out, "keys read"), _rows_view(v_out, "values read")
-        if k_out.shape != (n, n_kv * hd) or v_out.shape != k_out.shape or k_out.dtype != self.dtype or v_out.dtype != self.dtype:
-            raise KernelError(f"kv_read_int8: keys and values must be {self.dtype} [rows, {n_kv} x {hd}]")
-        self._rows_of_pages("kv_read_int8", n, row_seq, row_pos, page_table)
+        shape, dtype = k_out.shape, self.dtype
+        n, width = shape
+        if width != n_kv * hd or v_out.shape != shape or k_out.dtype is not dtype or v_out.dtype is not dtype:
+            raise KernelError(f"kv_read_int8: keys and values must be {dtype} [rows, {n_kv} x {hd}]")
+        reach = self._rows_of_pages("kv_read_int8", n, row_seq, row_pos, page_table)
         h = lib("int8_cache")
         _check(h.kvad_kv_read_int8(self.code, k_out.data_ptr(), v_out.data_ptr(), ld_k, ld_v, row_seq.data_ptr(), row_pos.data_ptr(), page_table.data_ptr(),
-                                   page_table.shape[1], k_pages.data_ptr(), k_scales.data_ptr(), v_pages.data_ptr(), v_scales.data_ptr(), n, n_kv, hd, page,
+                                   reach, k_pages.data_ptr(), k_scales.data_ptr(), v_pages.data_ptr(), v_scales.data_ptr(), n, n_kv, hd, page,
                                    _stream()), h)
 
     INT8_PROMPT_HEAD_SIZES = (16, 32, 48, 64, 80, 96, 112, 128)
@@ -1957,22 +1969,25 @@ class Ops:
         _need_cuda(q, out, seq_starts, kv_lens, page_table, k_pages, k_scales, v_pages, v_scales)
         ld_q, ld_o = _rows_view(q, "attention queries"), _rows_view(out, "attention output")
         _, n_kv, page, hd = self._int8_pages("attention_int8", k_pages, k_scales, v_pages, v_scales)
-        n = q.shape[0]
-        if q.shape[1] != n_heads * hd or out.shape != q.shape:
+        shape, dtype = q.shape, self.dtype
+        n = shape[0]
+        if shape[1] != n_heads * hd or out.shape != shape:
             raise KernelError("attention_int8: queries/output do not match heads x head size")
-        if q.dtype != self.dtype or out.dtype != self.dtype:
-            raise KernelError(f"attention_int8: queries and output must be {self.dtype}")
-        if (seq_starts.dtype != torch.int32 or kv_lens.dtype != torch.int32 or seq_starts.numel() <= n_seqs or kv_lens.numel() < n_seqs
-                or page_table.dtype != torch.int32 or page_table.dim() != 2 or not page_table.is_contiguous() or page_table.shape[0] < n_seqs):
+        if q.dtype is not dtype or out.dtype is not dtype:
+            raise KernelError(f"attention_int8: queries and output must be {dtype}")
+        i32, t_shape = torch.int32, page_table.shape
+        if (seq_starts.dtype is not i32 or kv_lens.dtype is not i32 or seq_starts.numel() <= n_seqs or kv_lens.numel() < n_seqs
+                or page_table.dtype is not i32 or len(t_shape) != 2 or not page_table.is_contiguous() or t_shape[0] < n_seqs):
             raise KernelError("attention_int8: starts, lengths and the page table are int32, an entry (and one start more) per sequence")
+        width = t_shape[1]
         if (max_new > 1 and self.dtype == torch.bfloat16 and hd in self.INT8_PROMPT_HEAD_SIZES and page == 64 and n_heads % n_kv == 0 and n_heads // n_kv <= 128
                 and ld_q % 8 == 0 and ld_o % 8 == 0
                 and (q.data_ptr() | out.data_ptr() | k_pages.data_ptr() | v_pages.data_ptr() | k_scales.data_ptr() | v_scales.data_ptr()) % 16 == 0):
-            parts, part_pages = self.int8_parts(n, n_seqs, n_kv, n_heads // n_kv, page_table.shape[1], window, keep_first)
+            parts, part_pages = self.int8_parts(n, n_seqs, n_kv, n_heads // n_kv, width, window, keep_first)
             scratch = torch.empty(n * n_heads * parts * (hd + 2), dtype=torch.float32, device=q.device) if parts > 1 else None
             h = lib("attention_int8_prompt")
             _check(h.kvad_attention_int8_prompt(q.data_ptr(), ld_q, out.data_ptr(), ld_o, seq_starts.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(),
-                                                page_table.shape[1], k_pages.data_ptr(), k_scales.data_ptr(), v_pages.data_ptr(), v_scales.data_ptr(), n,
+                                                width, k_pages.data_ptr(), k_scales.data_ptr(), v_pages.data_ptr(), v_scales.data_ptr(), n,
                                                 int(n_seqs), int(max_new), int(n_heads), n_kv, hd, page, float(scale), int(window or 0), int(keep_first or 0),
                                                 parts, part_pages, _ptr(scratch), _stream()), h)
             if parts > 1:
@@ -1980,13 +1995,13 @@ class Ops:
             return
         splits, split_pages, warps, scratch = 1, 0, 4, None
         if max_new == 1:
-            reach = page_table.shape[1] if not window else min(page_table.shape[1], -(-window // 64) + 1 + -(-keep_first // 64))
+            reach = width if not window else min(width, -(-window // 64) + 1 + -(-keep_first // 64))
             splits, split_pages, warps = self.int8_splits(n_seqs * n_kv * -(-(n_heads // n_kv) // 16), reach)
             if splits > 1:
                 scratch = torch.empty(n * n_heads * splits * (hd + 2), dtype=torch.float32, device=q.device)
         h = lib("attention_int8")
         _check(h.kvad_attention_int8(self.code, q.data_ptr(), ld_q, out.data_ptr(), ld_o, seq_starts.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(),
-                                     page_table.shape[1], k_pages.data_ptr(), k_scales.data_ptr(), v_pages.data_ptr(), v_scales.data_ptr(), k_pages.shape[0], n,
+                                     width, k_pages.data_ptr(), k_scales.data_ptr(), v_pages.data_ptr(), v_scales.data_ptr(), k_pages.shape[0], n,
                                      int(n_seqs), int(max_new), int(n_heads), n_kv, hd, page, float(scale), int(window or 0), int(keep_first or 0), splits,
                                      split_pages, warps, _ptr(scratch), _stream()), h)
         if splits > 1:
