@@ -2025,14 +2025,16 @@ class Ops:
     def int8_splits(items: int, reach: int, n_sms: Optional[int] = None) -> tuple:
         """How single-token rows deal out the pages of a sequence and key/value head (`items` of them, `reach` pages each at most): (blocks, pages a block,
         warps a block).  Up to as many items as SMs: blocks of eight warps, one an SM, whole rounds of their warps; up to 16 pages one block has them all (it takes
-        a second launch to join several).  More items: blocks of four warps, three an SM, with 48 pages at most, so that sequences of unequal lengths
+        a second launch to join several), with a warp for each up to twelve.  More items: blocks of four warps, three an SM, with 48 pages at most, so that sequences of unequal lengths
         keep all SMs busy.  (us, heads of 128 in fours, one sequence of 8000 positions, 8 heads: 8, 16, 32 pages for eight warps 13.5, 13.5, 17.5, for four
         14.3, 16.3, 21.8; of 30000: 36.8, 27.5, 21.6; 8 sequences of 4000: 32.1, 25.0, 20.4, all 26.5; 64 of 1000..8192: 32, 48 pages for four warps
-        115, 111, all for eight 115.  64 sequences of 520, 12 heads of 64: all for eight 23.2, for four 21.8; one of 520: 7.4, 8.2.)"""
+        115, 111, all for eight 115.  64 sequences of 520, 12 heads of 64: all for eight 27.4, for four 22.6; 8 of 520: twelve, eight, four warps 7.0, 8.3, 8.2, one 6.7, 7.2, 7.7.)"""
         sms = n_sms or sm_count()
         if items > sms:
             return -(-reach // 48), 48, 4
-        blocks = max(1, sms // max(1, items)) if reach > 16 else 1
+        if reach <= 16:
+            return 1, reach, min(reach, 12)
+        blocks = max(1, sms // max(1, items))
         pages = -(-reach // (8 * blocks)) * 8
         return -(-reach // pages), pages, 8
 
