@@ -10,7 +10,8 @@
 // A group of lanes (a power of two, head size / 8 at least) has one row, and of it one head's keys or values, or several heads' where there are many rows: a lane
 // brings eight entries, the group's maximum is a few shuffles, and the codes leave as eight bytes a lane.  Where a row goes is looked up once for these heads
 // (a chain of two trips to memory), and all their entries are asked for before the first is worked on.  Bound by memory, entry + 1 bytes
-// a code: 26289 bfloat16 rows of 8 heads of 128 are stored in 41 us (3.9 TB/s; four rows of one head a group: 79) and read in 30 (5.5 TB/s).
+// a code: 26289 bfloat16 rows of 8 heads of 128 are stored in 37 us (4.4 TB/s; four heads, turned to 32-bit on arrival: 41; four rows of one head a group: 79) and read in 30
+// (5.5 TB/s).
 //
 // No pointer is __restrict__: what is promised not to change may be read before the wait for the kernel that writes it.
 #include <type_traits>
