@@ -253,8 +253,21 @@ attention_int8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 #pragma unroll
       for (int n = 0; n < NT; ++n) sc[m][n][0] = sc[m][n][1] = sc[m][n][2] = sc[m][n][3] = 0.f;
     constexpr int STEPS = KS < 2 ? 1 : 2, TILES = 2 / STEPS;     // four matrices a load: two halves of 16 keys, of two steps or of two sixteens of keys
+    // (in 32-bit 64 entries' products have an accumulator of their own, for the reason given at the outputs)
+    constexpr int RUN = PIECES == 2 && KS > 4 ? 4 : KS;
+    float run[RUN < KS ? 4 : 1][NT][4];
+    auto acc = [&](int m, int n) -> float(&)[4] { return RUN < KS ? run[RUN < KS ? m : 0][n] : sc[m][n]; };
 #pragma unroll
     for (int s0 = 0; s0 < KS; s0 += STEPS) {
+      if (RUN < KS && s0 % RUN == 0) {
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float(&x)[4] = acc(m, n);
+            x[0] = x[1] = x[2] = x[3] = 0.f;
+          }
+      }
       uint32_t w[4][4];
 #pragma unroll
       for (int m = 0; m < 4; m += TILES)
@@ -274,8 +287,18 @@ attention_int8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int p = PIECES - 1; p >= 0; --p) mma_f16(sc[m][n], a0, a1, a2, a3, q[p][n]);
+            for (int p = PIECES - 1; p >= 0; --p) mma_f16(acc(m, n), a0, a1, a2, a3, q[p][n]);
         }
+      }
+      if (RUN < KS && (s0 + STEPS) % RUN == 0) {
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const float(&x)[4] = acc(m, n);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[m][n][e] += x[e];
+          }
       }
     }
     // scores in powers of two

@@ -76,7 +76,8 @@ def test_a_row_that_is_not_finite_says_so_and_leaves_the_others_alone(bad, width
 
 
 @pytest.mark.parametrize("norm", ["rms", "layer"])
-@pytest.mark.parametrize("n,width,extra", [(1, 16, 0), (8, 1024, 0), (3, 1600, 0), (5, 257, 0), (4, 300, 3), (9, 77, 1), (2, 6400, 8), (1, 20000, 0)])
+@pytest.mark.parametrize("n,width,extra", [(1, 16, 0), (8, 1024, 0), (3, 1600, 0), (5, 257, 0), (4, 300, 3), (9, 77, 1), (2, 6400, 8), (1, 20000, 0), (149, 700, 0), (150, 1500, 0), (149, 2048, 0), (151, 3000, 0), (149, 4096, 0), (149, 6000, 0), (149, 8192, 0),
+                                           (149, 16000, 0), (2, 4096, 0), (2, 8000, 0)])
 @pytest.mark.parametrize("params", ["float32", "bfloat16", None])
 @pytest.mark.parametrize("delta", [None, "float32", "bfloat16"])
 def test_normed_rows(norm, n, width, extra, params, delta):
@@ -359,7 +360,7 @@ def check_attention(dtype, new, before, n_heads, kv_heads, hd, window=0, keep_fi
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
 @pytest.mark.parametrize("n_heads,kv_heads,hd", [(2, 2, 16), (4, 1, 32), (3, 3, 48), (12, 12, 64), (8, 2, 64), (6, 2, 80), (3, 1, 96), (2, 1, 112), (8, 2, 128), (4, 4, 128),
                                                  (5, 1, 144), (16, 1, 64), (20, 1, 128), (2, 2, 192), (4, 2, 256)])
-@pytest.mark.parametrize("before", [[0], [62, 63, 64, 65, 0, 300], [1500, 3, 700]])
+@pytest.mark.parametrize("before", [[0], [62, 63, 64, 65, 0, 300], [700, 650], [1500, 3, 700]])
 def test_attention_of_single_tokens(dtype, n_heads, kv_heads, hd, before):
     check_attention(dtype, [1] * len(before), before, n_heads, kv_heads, hd, lead=8)
 
@@ -398,6 +399,16 @@ def test_a_sequence_without_new_rows(dtype):
 def test_long_contexts(dtype, new):
     check_attention(dtype, [new], [9000], 4, 2, 128)
     check_attention(dtype, [new, new], [6000, 40], 2, 2, 64, spread=6.0)
+
+
+@pytest.mark.parametrize("seqs,longest,n_heads,kv_heads,hd,window", [(40, 200, 8, 4, 64, 0), (33, 300, 8, 8, 128, 0), (40, 200, 4, 4, 64, 100), (260, 4, 2, 1, 16, 0), (300, 1, 2, 2, 64, 0)])
+def test_more_blocks_than_multiprocessors(seqs, longest, n_heads, kv_heads, hd, window):
+    """Blocks come in the order of the pages they see, which each finds for itself (up to 256 sequences); some sequences have no new rows."""
+    g = torch.Generator().manual_seed(seqs)
+    new = [int(x) for x in torch.randint(0, longest + 1, (seqs,), generator=g)]
+    new[3], new[5] = longest, 0
+    before = [int(x) + (n == 0) for x, n in zip(torch.randint(0, 700, (seqs,), generator=g), new)]
+    check_attention("bfloat16", new, before, n_heads, kv_heads, hd, window)
 
 
 @pytest.mark.parametrize("new", [[1, 1], [80, 1]])
