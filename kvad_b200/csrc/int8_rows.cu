@@ -11,8 +11,9 @@
 //
 // One pass: a row's entries stay in the registers of its threads from the sum through both reductions (mean square, maximum) to the
 // codes.  Sums, norms and scales are 32-bit; the only rounding to fewer bits is the code itself.  Bound by memory: 16384 rows of 4096, RMS norm after a sum with
-// bfloat16 results, 113 us (6.5 TB/s; 11 bytes an entry); without the sum 72 (4.7), layer norm 88 (3.8), bfloat16 rows as they are 45 (4.5), where a row's reductions leave
-// its block with nothing in flight (a block that asked for its next row beforehand was slower: 103 for the layer norm; so many registers leave fewer blocks).
+// bfloat16 results, 111 to 113 us (6.5 TB/s; 11 bytes an entry); without the sum 66 (5.1), layer norm 71 (4.7), bfloat16 rows as they are 43 (4.7), where a row's reductions leave
+// its block with nothing in flight (blocks that asked for their next row beforehand were slower, 103 for the layer norm, and so were rows fetched ahead into the L2, 93: it is
+// the instructions' latencies, not memory's).
 // kvad_int8_read: codes back to numbers.
 //
 // No pointer is __restrict__: what is promised not to change may be read before the wait for the kernel that writes it.
@@ -31,9 +32,6 @@ __device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_ca
 __device__ __forceinline__ float4 load4(const __nv_bfloat16* p) {
   const uint2 q = *reinterpret_cast<const uint2*>(p);
   return make_float4(__uint_as_float(q.x << 16), __uint_as_float(q.x & 0xffff0000u), __uint_as_float(q.y << 16), __uint_as_float(q.y & 0xffff0000u));
-}
-__device__ __forceinline__ float4 load4_param(const void* p, int64_t i, int is_f32) {
-  return is_f32 ? load4(reinterpret_cast<const float*>(p) + i) : load4(reinterpret_cast<const __nv_bfloat16*>(p) + i);
 }
 __device__ __forceinline__ void store4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
 __device__ __forceinline__ void store4(__nv_bfloat16* p, float4 v) {
@@ -68,10 +66,10 @@ template <int TPR> __device__ __forceinline__ uint32_t row_max(uint32_t v, float
 
 // TPR threads a row, 4 * V entries a thread at most.  VEC: four entries at a time (every row on a 4-entry boundary), else one.
 template <typename T, int NORM, int TPR, int V, bool VEC>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, V > 4 ? 1 : 1536 / (TPR < 128 ? 128 : TPR))
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, V > 4 ? (TPR > 512 ? 1 : 896 / TPR) : 1536 / (TPR < 128 ? 128 : TPR))
 int8_rows_kernel(const T* x, int64_t ld_x, const int* rows, const void* delta, int delta_f32, int64_t ld_delta,
                  float mult, float* x_out, int64_t ld_out, const void* weight, const void* bias, int params_f32,
-                 int unit_offset, int8_t* codes, int64_t ld_codes, float* scales, int n, int width, float eps) {
+                 int unit_offset, int8_t* codes, int64_t ld_codes, float* scales, int n, int width, float inv_width, float eps) {
   constexpr int BLOCK = TPR < 128 ? 128 : TPR;
   __shared__ float scratch[TPR == 32 ? 1 : TPR / 32];
   // (what rows without a norm become may be weights, which the products fetch before they wait for the kernel before them: no early start there)
@@ -96,19 +94,25 @@ int8_rows_kernel(const T* x, int64_t ld_x, const int* rows, const void* delta, i
     }
   }
   if (NORM != NORM_NONE) {
+    // (which type a parameter has is asked once, not entry by entry)
     if (delta != nullptr) {
+      auto add = [&](auto* d) {
+        d += src * ld_delta;
 #pragma unroll
-      for (int e = 0; e < 4 * V; e += VEC ? 4 : 1) {
-        const int j = place(e);
-        if (j < width) {
-          if (VEC) {
-            const float4 d = load4_param(delta, src * ld_delta + j, delta_f32);
-            v[e] = fmaf(mult, d.x, v[e]); v[e + 1] = fmaf(mult, d.y, v[e + 1]); v[e + 2] = fmaf(mult, d.z, v[e + 2]); v[e + 3] = fmaf(mult, d.w, v[e + 3]);
-          } else {
-            v[e] = fmaf(mult, load_param(delta, src * ld_delta + j, delta_f32), v[e]);
+        for (int e = 0; e < 4 * V; e += VEC ? 4 : 1) {
+          const int j = place(e);
+          if (j < width) {
+            if (VEC) {
+              const float4 q = load4(d + j);
+              v[e] = fmaf(mult, q.x, v[e]); v[e + 1] = fmaf(mult, q.y, v[e + 1]); v[e + 2] = fmaf(mult, q.z, v[e + 2]); v[e + 3] = fmaf(mult, q.w, v[e + 3]);
+            } else {
+              v[e] = fmaf(mult, to_f32(d[j]), v[e]);
+            }
           }
         }
-      }
+      };
+      if (delta_f32) add(reinterpret_cast<const float*>(delta));
+      else add(reinterpret_cast<const __nv_bfloat16*>(delta));
     }
     if (x_out != nullptr) {
 #pragma unroll
@@ -120,36 +124,43 @@ int8_rows_kernel(const T* x, int64_t ld_x, const int* rows, const void* delta, i
         }
       }
     }
-    const float inv_width = 1.f / (float)width;
     if (NORM == NORM_LAYER) {
       float sum = 0.f;
 #pragma unroll
       for (int e = 0; e < 4 * V; ++e) sum += v[e];
       const float mean = row_sum<TPR>(sum, scratch) * inv_width;
 #pragma unroll
-      for (int e = 0; e < 4 * V; ++e) v[e] = place(e) < width ? v[e] - mean : 0.f;
+      for (int e = 0; e < 4 * V; e += VEC ? 4 : 1)
+        if (place(e) < width) {
+#pragma unroll
+          for (int i = 0; i < (VEC ? 4 : 1); ++i) v[e + i] -= mean;
+        }
     }
     float sq = 0.f;
 #pragma unroll
     for (int e = 0; e < 4 * V; ++e) sq = fmaf(v[e], v[e], sq);
-    const float rstd = 1.f / sqrtf(row_sum<TPR>(sq, scratch) * inv_width + eps);
+    const float var = row_sum<TPR>(sq, scratch) * inv_width + eps, guess = rsqrtf(var);
+    const float rstd = var > 1e-30f && var < 1e30f ? fmaf(fmaf(-var * guess, guess, 1.f) * 0.5f, guess, guess) : 1.f / sqrtf(var);      // (a Newton step: to the last place or two)
+    const float one = unit_offset ? 1.f : 0.f;
+    auto weigh = [&](auto* w, auto* b) {
 #pragma unroll
-    for (int e = 0; e < 4 * V; e += VEC ? 4 : 1) {
-      const int j = place(e);
-      if (j < width) {
-        if (VEC) {
-          float4 w = make_float4(1.f, 1.f, 1.f, 1.f), b = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (weight != nullptr) w = load4_param(weight, j, params_f32);
-          if (bias != nullptr) b = load4_param(bias, j, params_f32);
-          const float one = unit_offset ? 1.f : 0.f;
-          v[e] = fmaf(v[e] * rstd, w.x + one, b.x); v[e + 1] = fmaf(v[e + 1] * rstd, w.y + one, b.y);
-          v[e + 2] = fmaf(v[e + 2] * rstd, w.z + one, b.z); v[e + 3] = fmaf(v[e + 3] * rstd, w.w + one, b.w);
-        } else {
-          const float w = (weight != nullptr ? load_param(weight, j, params_f32) : 1.f) + (unit_offset ? 1.f : 0.f);
-          v[e] = fmaf(v[e] * rstd, w, bias != nullptr ? load_param(bias, j, params_f32) : 0.f);
+      for (int e = 0; e < 4 * V; e += VEC ? 4 : 1) {
+        const int j = place(e);
+        if (j < width) {
+          if (VEC) {
+            float4 x = make_float4(1.f, 1.f, 1.f, 1.f), y = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (w != nullptr) x = load4(w + j);
+            if (b != nullptr) y = load4(b + j);
+            v[e] = fmaf(v[e] * rstd, x.x + one, y.x); v[e + 1] = fmaf(v[e + 1] * rstd, x.y + one, y.y);
+            v[e + 2] = fmaf(v[e + 2] * rstd, x.z + one, y.z); v[e + 3] = fmaf(v[e + 3] * rstd, x.w + one, y.w);
+          } else {
+            v[e] = fmaf(v[e] * rstd, (w != nullptr ? to_f32(w[j]) : 1.f) + one, b != nullptr ? to_f32(b[j]) : 0.f);
+          }
         }
       }
-    }
+    };
+    if (params_f32) weigh(reinterpret_cast<const float*>(weight), reinterpret_cast<const float*>(bias));
+    else weigh(reinterpret_cast<const __nv_bfloat16*>(weight), reinterpret_cast<const __nv_bfloat16*>(bias));
   }
   float most = 0.f;
 #pragma unroll
@@ -226,23 +237,33 @@ template <typename T, int NORM, int TPR, int V, bool VEC> cudaError_t go(const C
   const int per_block = BLOCK / TPR;
   return kvad_launch(int8_rows_kernel<T, NORM, TPR, V, VEC>, dim3((unsigned)((c.n + per_block - 1) / per_block)), dim3(BLOCK), 0, c.stream,
                      reinterpret_cast<const T*>(c.x), c.ld_x, c.rows, c.delta, c.delta_f32, c.ld_delta, c.mult, c.x_out, c.ld_out, c.weight, c.bias,
-                     c.params_f32, c.unit_offset, c.codes, c.ld_codes, c.scales, c.n, c.width, c.eps);
+                     c.params_f32, c.unit_offset, c.codes, c.ld_codes, c.scales, c.n, c.width, 1.f / (float)c.width, c.eps);
 }
 
-// Threads for a row: a warp up to 512 entries (no barriers), then as many as give each 16 entries, then 32; of the pieces that a thread could have, no more than
-// the width needs.
+// Threads for a row.  Many rows: a warp up to 512 entries (no barriers), then so many that each has up to 32 entries, which is what covers the cost of a row's reductions: some 220 instructions a
+// thread (layer norm of 16384 rows of 4096: 71 us with 32 entries a thread, 79 with 16).  Up to a row an SM: 4 to 8 entries a thread, since a row is then a
+// chain of waits (RMS norm of 8 rows of 1600: 2.1 us against 2.7, of 4096 2.6 against 4.1; of 256 rows of 1024 2.7 against 2.4).  Of the pieces that a thread could have, no more
+// than the width needs.
+constexpr int FEW = 148;
+
 template <typename T, int NORM, bool VEC> cudaError_t by_width(const Call& c) {
   if (c.width <= 128) return go<T, NORM, 32, 1, VEC>(c);
   if (c.width <= 256) return go<T, NORM, 32, 2, VEC>(c);
   if (c.width <= 512) return go<T, NORM, 32, 4, VEC>(c);
+  if (c.n <= FEW && VEC) {
+    if (c.width <= 1024) return go<T, NORM, 256, 1, VEC>(c);
+    if (c.width <= 2048) return go<T, NORM, 512, 1, VEC>(c);
+    if (c.width <= 4096) return go<T, NORM, 512, 2, VEC>(c);
+    if (c.width <= 8192) return go<T, NORM, 1024, 2, VEC>(c);
+  }
   if (c.width <= 1024) return go<T, NORM, 128, 2, VEC>(c);
   if (c.width <= 1536) return go<T, NORM, 128, 3, VEC>(c);
   if (c.width <= 2048) return go<T, NORM, 128, 4, VEC>(c);
-  if (c.width <= 256 * 12) return go<T, NORM, 256, 3, VEC>(c);
-  if (c.width <= 4096) return go<T, NORM, 256, 4, VEC>(c);
-  if (c.width <= 512 * 12) return go<T, NORM, 512, 3, VEC>(c);
-  if (c.width <= 8192) return go<T, NORM, 512, 4, VEC>(c);
-  if (c.width <= 16384) return go<T, NORM, 1024, 4, VEC>(c);
+  if (c.width <= 128 * 24) return go<T, NORM, 128, 6, VEC>(c);
+  if (c.width <= 4096) return go<T, NORM, 128, 8, VEC>(c);
+  if (c.width <= 256 * 24) return go<T, NORM, 256, 6, VEC>(c);
+  if (c.width <= 8192) return go<T, NORM, 256, 8, VEC>(c);
+  if (c.width <= 16384) return go<T, NORM, 512, 8, VEC>(c);
   return go<T, NORM, 1024, 8, VEC>(c);
 }
 
