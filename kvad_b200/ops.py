@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 import os
 from ctypes import c_float, c_int, c_int64, c_uint, c_void_p
 from typing import Optional
@@ -393,6 +394,26 @@ def _scored_prompt_takes(dk: int, dv: int, alias: bool, out_f32: bool) -> bool:
 @functools.lru_cache(maxsize=256)
 def _scored_wide_takes(dk: int, dv: int, alias: bool) -> bool:
     return lib("attention_scored_wide").kvad_attention_scored_wide_takes(dk, dv, int(alias)) == 1
+
+
+@functools.lru_cache(maxsize=1024)
+def _int8_short(items: int, reach: int, hd: int, wide: bool, sms: int) -> int:
+    """Warps a block, which has all of a short context's pages: those with the fewest (rounds of pages + 2, for the start and the warps' meeting) x (waves of blocks), as many blocks at a time
+    as the SMs have shared memory and registers for.  (us, contexts of 9 pages, three, four, five, eight, twelve warps: 8 items of 64 7.0 with twelve; 200 items 10.5, 10.4, 8.7, 9.5,
+    12.5; 384 14.6, 13.5, 12.5, 18.7, 20.9; 1600 32.9, 34.6, 36.7, 49, 70; heads of 128: 256 items 17.6, 16.2, 14.6, 20.6, 20.0; 512 20.6, 28.5, 25.8, 36.5, 34.9.)"""
+    padded = max(16, 1 << (hd - 1).bit_length())
+    page = -(-(2 * 64 * padded + 512) // 1024) * 1024
+    registers, most = (248, 8) if wide or padded > 128 else (168, 12) if padded > 64 else (128, 12)
+    best = None
+    for warps in range(1, min(reach, most) + 1):
+        an_sm = min(227 * 1024 // (warps * page + 4096), 65536 // (warps * 32 * registers))
+        if an_sm == 0:
+            break
+        waves = items / (sms * an_sm)
+        cost = (max(1.0, waves) + max(1, math.ceil(waves))) * (-(-reach // warps) + 2)      # (a wave that is begun counts half)
+        if best is None or cost < best[0] or (cost == best[0] and items <= sms):
+            best = (cost, warps)
+    return best[1] if best else 1
 
 
 class Ops:
@@ -1996,7 +2017,8 @@ class Ops:
         splits, split_pages, warps, scratch = 1, 0, 4, None
         if max_new == 1:
             reach = width if not window else min(width, -(-window // 64) + 1 + -(-keep_first // 64))
-            splits, split_pages, warps = self.int8_splits(n_seqs * n_kv * -(-(n_heads // n_kv) // 16), reach)
+            group = n_heads // n_kv
+            splits, split_pages, warps = self.int8_splits(n_seqs * n_kv * -(-group // 16), reach, hd, group > 8)
             if splits > 1:
                 scratch = torch.empty(n * n_heads * splits * (hd + 2), dtype=torch.float32, device=q.device)
         h = lib("attention_int8")
@@ -2022,18 +2044,18 @@ class Ops:
         return -(-reach // pages), pages
 
     @staticmethod
-    def int8_splits(items: int, reach: int, n_sms: Optional[int] = None) -> tuple:
-        """How single-token rows deal out the pages of a sequence and key/value head (`items` of them, `reach` pages each at most): (blocks, pages a block,
-        warps a block).  Up to as many items as SMs: blocks of eight warps, one an SM, whole rounds of their warps; up to 16 pages one block has them all (it takes
-        a second launch to join several), with a warp for each up to twelve.  More items: blocks of four warps, three an SM, with 48 pages at most, so that sequences of unequal lengths
-        keep all SMs busy.  (us, heads of 128 in fours, one sequence of 8000 positions, 8 heads: 8, 16, 32 pages for eight warps 13.5, 13.5, 17.5, for four
-        14.3, 16.3, 21.8; of 30000: 36.8, 27.5, 21.6; 8 sequences of 4000: 32.1, 25.0, 20.4, all 26.5; 64 of 1000..8192: 32, 48 pages for four warps
-        115, 111, all for eight 115.  64 sequences of 520, 12 heads of 64: all for eight 27.4, for four 22.6; 8 of 520: twelve, eight, four warps 7.0, 8.3, 8.2, one 6.7, 7.2, 7.7.)"""
+    def int8_splits(items: int, reach: int, hd: int = 64, wide: bool = False, n_sms: Optional[int] = None) -> tuple:
+        """How single-token rows deal out the pages of a sequence and key/value head (`items` of them, `reach` pages each at most; `wide`: more than eight query heads
+        share a key/value head): (blocks, pages a block, warps a block).  Up to 16 pages one block has them all (it takes a second launch to join several): see `_int8_short`.
+        Up to as many items as SMs: blocks of eight warps, one an SM, whole rounds of their warps.  More items: blocks of four warps, three an SM, with 48 pages at most, so
+        that sequences of unequal lengths keep all SMs busy.  (us, heads of 128 in fours, one sequence of 8000 positions, 8 heads: 8, 16, 32 pages for eight warps 13.5, 13.5,
+        17.5, for four 14.3, 16.3, 21.8; of 30000: 36.8, 27.5, 21.6; 8 sequences of 4000: 32.1, 25.0, 20.4, all 26.5; 64 of 1000..8192: 32, 48, 64 pages for four warps
+        116, 111, 121, all for eight 111.)"""
         sms = n_sms or sm_count()
+        if reach <= 16:
+            return 1, reach, _int8_short(items, reach, hd, wide, sms)
         if items > sms:
             return -(-reach // 48), 48, 4
-        if reach <= 16:
-            return 1, reach, min(reach, 12)
         blocks = max(1, sms // max(1, items))
         pages = -(-reach // (8 * blocks)) * 8
         return -(-reach // pages), pages, 8

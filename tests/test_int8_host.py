@@ -57,9 +57,10 @@ def test_storage_of_a_group_in_8_bits():
 
 @pytest.mark.parametrize("items,reach", [(1, 1), (12, 9), (96, 16), (96, 17), (8, 126), (8, 471), (148, 40), (149, 16), (512, 129), (4000, 3)])
 def test_every_page_goes_to_one_block(items, reach):
-    blocks, pages, warps = Ops.int8_splits(items, reach, n_sms=148)
-    assert 1 <= warps <= 12 and blocks >= 1 and (blocks - 1) * pages < reach <= blocks * pages
-    assert reach > 16 or blocks == 1
+    for hd, wide in ((16, False), (64, False), (128, False), (128, True), (256, False)):
+        blocks, pages, warps = Ops.int8_splits(items, reach, hd, wide, n_sms=148)
+        assert 1 <= warps <= 12 and blocks >= 1 and (blocks - 1) * pages < reach <= blocks * pages
+        assert reach > 16 or blocks == 1
 
 
 @pytest.mark.parametrize("rows,seqs,kv,group,width,window", [(2048, 2, 16, 1, 16, 0), (330, 2, 2, 4, 43, 0), (5, 1, 2, 4, 126, 0), (5, 1, 1, 128, 126, 0), (300, 1, 4, 2, 500, 100)])
