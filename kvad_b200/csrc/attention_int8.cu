@@ -107,6 +107,7 @@ template <int HDP> __device__ __forceinline__ uint32_t place(int row, int c) {
   return (c >> 3) * (PAGE * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
 }
 
+// (twelve warps at most; 512 threads for the smaller heads: 128 registers a thread, so that an SM has room for four blocks of four warps)
 template <typename T, int HDP, int NT>
 __global__ void __launch_bounds__(NT == 1 && HDP <= 64 ? 512 : NT == 1 && HDP <= 128 ? 384 : 256, 1)
 attention_int8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Args a) {
@@ -518,7 +519,7 @@ int launch(const Args& a, const int8_t* k, const int8_t* v, int64_t cache_rows, 
   if (rc == KVAD_OK) rc = tensor_map(v, cache_rows, a.hd, L::PITCH, &mv);
   if (rc != KVAD_OK) return rc;
   auto kernel = attention_int8_kernel<T, HDP, NT>;
-  constexpr int MOST = NT == 1 && HDP <= 64 ? 16 : NT == 1 && HDP <= 128 ? 12 : 8;
+  constexpr int MOST = NT == 1 && HDP <= 128 ? 12 : 8;
   warps = warps < MOST ? warps : MOST;
   while (warps > 1 && L::smem(warps) > 227 * 1024) --warps;
   static bool configured = false;
@@ -554,7 +555,7 @@ int by_size(const Args& a, const int8_t* k, const int8_t* v, int64_t cache_rows,
 }  // namespace
 
 // `splits` > 1: the pages that a row sees are dealt out to that many blocks, `split_pages` each, through `scratch` (float32, rows x heads x splits x (head size + 2));
-// `warps`: of a block, up to 16 (fewer where a head's pages are too large).
+// `warps`: of a block, up to 12 (fewer where a head's pages are too large).
 KVAD_EXPORT int kvad_attention_int8(int dtype, const void* q, int64_t ld_q, void* out, int64_t ld_o, const int* seq_starts, const int* kv_lens,
                                     const int* table, int table_width, const int8_t* k_pages, const float* k_scales, const int8_t* v_pages,
                                     const float* v_scales, int n_pages, int n_rows, int n_seqs, int max_new, int n_heads, int kv_heads, int hd, int page,
@@ -566,7 +567,7 @@ KVAD_EXPORT int kvad_attention_int8(int dtype, const void* q, int64_t ld_q, void
   KVAD_REQUIRE(((reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages) | reinterpret_cast<uintptr_t>(k_scales) |
                  reinterpret_cast<uintptr_t>(v_scales)) & 15) == 0, "attention_int8: pages and scales must start on a 16-byte boundary");
   KVAD_REQUIRE(window >= 0 && keep_first >= 0, "attention_int8: a window and kept first positions cannot be negative");
-  KVAD_REQUIRE(warps >= 1 && warps <= 16 && splits >= 1 && (splits == 1 || (split_pages > 0 && scratch != nullptr)), "attention_int8: no way to deal out pages: %d, %d, %d",
+  KVAD_REQUIRE(warps >= 1 && warps <= 12 && splits >= 1 && (splits == 1 || (split_pages > 0 && scratch != nullptr)), "attention_int8: no way to deal out pages: %d, %d, %d",
                splits, split_pages, warps);
   const int64_t cache_rows = (int64_t)n_pages * kv_heads * PAGE;
   KVAD_REQUIRE(cache_rows < (1ll << 31), "attention_int8: more cached rows than a copy can name");
