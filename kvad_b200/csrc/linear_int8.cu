@@ -4,9 +4,9 @@
 //
 // Many rows: the 5th-generation tensor cores (tcgen05.mma.kind::i8, 32-bit whole-number accumulators in tensor memory).  Both operands are K-major
 // and come by TMA in blocks of 128 entries of K (one row of the 128-byte swizzle); a CTA computes tiles of 128 x BN, one after another, the
-// epilogue of one under the products of the next (two accumulators); results leave by TMA through slabs of 32 rows x 64 bytes a warp, two in turn.  Bound by the tensor cores where K is
-// long: 8192 x 8192 x 4096 with 32-bit results 204 to 230 us (2.4 to 2.7 POP/s, 73 to 82 % of twice the measured bfloat16 rate, at the power limit), and by first loads and last epilogues where a CTA
-// has few tiles: 2048 x 6400 x 1600 21.0 us, with tanh GELU 23.5 (12.8 by its operations; 34.4 with results written by the threads).
+// epilogue of one under the products of the next (two accumulators), or a pair of CTAs tiles of 256 x 256 (see tile_width); results leave by TMA through slabs of 32 rows x 64 bytes a warp, two in turn.  Bound by the tensor cores where K is
+// long: 8192 x 8192 x 4096 189 us (2.9 POP/s, 89 % of twice the measured bfloat16 rate, at the power limit), with 32-bit results 200 to 220, and by first loads and last epilogues where a CTA
+// has few tiles: 2048 x 6400 x 1600 19.1 us, with tanh GELU 23.3 (12.8 by its operations; 34.4 with results written by the threads).
 //
 // Few rows: a stream of weights, bound by their bytes (8 rows into 50257 outputs of 1600 entries: 18.9 us, 4.3 TB/s) and in small products by a launch and one
 // trip to memory (into 4800 outputs: 4.1 us).  A CTA has 16 outputs; its warps share K in pieces of 64 entries, of which a lane brings 16 contiguous
@@ -137,8 +137,9 @@ linear_int8_few_kernel(const int8_t* a, int64_t lda, const int8_t* __restrict__ 
 constexpr int BM = 128, BK = 128;             // 128 entries of K: one row of the 128-byte swizzle
 constexpr int THREADS = 320;                  // warp 0: TMA, warp 1: products and tensor memory, warps 2-9: epilogue
 
-template <int BN> struct Tile {
-  static constexpr uint32_t A_BYTES = BM * BK, B_BYTES = BN * BK;
+// PAIR: two CTAs on a tile of 256 x BN, each with 128 rows and half of the weights; the tensor cores of both read both halves.
+template <int BN, bool PAIR> struct Tile {
+  static constexpr uint32_t A_BYTES = BM * BK, B_BYTES = (PAIR ? BN / 2 : BN) * BK;
   static constexpr int STAGES_RAW = 192 * 1024 / (A_BYTES + B_BYTES);
   static constexpr int STAGES = STAGES_RAW > 8 ? 8 : STAGES_RAW;
   static constexpr uint32_t OFF_SLAB = STAGES * (A_BYTES + B_BYTES);        // two of 2 KB an epilogue warp: 32 rows x 64 bytes of output on their way out by TMA
@@ -159,6 +160,36 @@ __device__ __forceinline__ void umma_i8(uint32_t d, uint64_t a_desc, uint64_t b_
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
       ::"r"(d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(zero) : "memory");
+}
+
+__device__ __forceinline__ void umma_i8_pair(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+// Arrives on the barrier at this place in both CTAs of the pair once everything issued before has run.
+__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
+}
+// The place that `p` has in this CTA, in the first CTA of the pair.
+__device__ __forceinline__ uint32_t in_first(const void* p) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(0));
+  return r;
+}
+// Into this CTA's memory, counted by a barrier of the first CTA's.
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+               ::"r"(smem_u32(dst)), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity) {
+  const uint32_t limit = g_wait_limit;
+  for (uint32_t i = 0; i < limit; ++i)
+    if (mbar_try_wait_cluster(bar, parity)) return true;
+  atomicAdd(&g_wait_timeouts, 1);
+  return false;
 }
 
 // Asks for columns of a row in tensor memory, and waits for them.  (The registers go through the wait, so that nothing that works on them comes before it.)
@@ -191,12 +222,12 @@ __device__ __forceinline__ void put_all(const Out& o, int row, int n, int N, con
     if (n + j < N) put<T, EPI>(o, (int64_t)row * o.ld + n + j, v[j]);
 }
 
-template <typename T, int EPI, int BN>
+template <typename T, int EPI, int BN, bool PAIR>
 __global__ void __launch_bounds__(THREADS, 1)
 linear_int8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_out,
                    int tma_out, Out o, int M, int N, int K, int skip_copy) {
-  using L = Tile<BN>;
-  constexpr int STAGES = L::STAGES;
+  using L = Tile<BN, PAIR>;
+  constexpr int STAGES = L::STAGES, ROWS = PAIR ? 2 * BM : BM;
   constexpr uint32_t TMEM = 2 * BN;             // two accumulators (a power of two)
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* a_tiles = smem;
@@ -204,7 +235,7 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
   uint64_t* empty = full + STAGES;
   uint64_t* acc_full = empty + STAGES;          // [2] the accumulator is complete
-  uint64_t* acc_empty = acc_full + 2;           // [2] the eight epilogue warps have read it
+  uint64_t* acc_empty = acc_full + 2;           // [2] the eight epilogue warps have read it (of the first CTA: both CTAs')
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile uint32_t* gave_up = tmem_slot + 1;
   float* col_scale = reinterpret_cast<float*>(smem + L::OFF_COLS);
@@ -212,7 +243,8 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
 
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tiles_n = (N + BN - 1) / BN, n_tiles = tiles_n * ((M + BM - 1) / BM), n_kb = (K + BK - 1) / BK;
+  const int tiles_n = (N + BN - 1) / BN, n_tiles = tiles_n * ((M + ROWS - 1) / ROWS), n_kb = (K + BK - 1) / BK;
+  const int rank = PAIR ? blockIdx.x & 1 : 0, first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
   if (threadIdx.x == 0) {
     prefetch_tensormap(&map_a);
     prefetch_tensormap(&map_w);
@@ -223,15 +255,23 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 8);
+      mbar_init(&acc_empty[b], PAIR ? 16 : 8);
     }
     *gave_up = (smem_u32(smem) & 1023) != 0;      // (the swizzle's rows start on 1024 bytes; the memory is asked for so)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  if (warp == 1) tmem_alloc(tmem_slot, TMEM);
+  if (warp == 1) {
+    if (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      tmem_alloc(tmem_slot, TMEM);
+    }
+  }
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync_all();                 // the other CTA's barriers are there before anything arrives on them
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   bool ok = *gave_up == 0;
@@ -240,37 +280,44 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     if (lane == 0) {
       uint32_t it = 0;                          // stages filled so far, over all tiles
       int asked = 0;                            // of the first tile: weights on the way before the kernel before has finished
-      for (int t = blockIdx.x; t < n_tiles && ok; t += gridDim.x) {
-        const int n0 = t % tiles_n * BN, m0 = t / tiles_n * BM;
-        if (t == (int)blockIdx.x) {
+      auto expect = [&](int s) {
+        if (rank == 0) mbar_expect_tx(&full[s], (PAIR ? 2 : 1) * (L::A_BYTES + L::B_BYTES));
+      };
+      auto load = [&](uint8_t* dst, const CUtensorMap* map, int s, int x, int y) {
+        if (PAIR) tma_load_pair(dst, map, in_first(&full[s]), x, y);
+        else tma_load_2d(dst, map, &full[s], x, y);
+      };
+      for (int t = first; t < n_tiles && ok; t += step) {
+        const int n0 = t % tiles_n * BN + rank * (BN / 2), m0 = t / tiles_n * ROWS + rank * BM;
+        if (t == first) {
           asked = n_kb < STAGES ? n_kb : STAGES;
           for (int i = 0; i < asked; ++i) {
-            mbar_expect_tx(&full[i], L::A_BYTES + L::B_BYTES);
-            if (!(skip_copy && i == 0)) tma_load_2d(b_tiles + i * L::B_BYTES, &map_w, &full[i], i * BK, n0);
+            expect(i);
+            if (!(skip_copy && i == 0)) load(b_tiles + i * L::B_BYTES, &map_w, i, i * BK, n0);
           }
           pdl_wait();
-          for (int i = 0; i < asked; ++i) tma_load_2d(a_tiles + i * L::A_BYTES, &map_a, &full[i], i * BK, m0);
+          for (int i = 0; i < asked; ++i) load(a_tiles + i * L::A_BYTES, &map_a, i, i * BK, m0);
           it = asked;
         }
-        for (int i = t == (int)blockIdx.x ? asked : 0; i < n_kb; ++i, ++it) {
+        for (int i = t == first ? asked : 0; i < n_kb; ++i, ++it) {
           const int s = it % STAGES;
           if (it >= (uint32_t)STAGES && !mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1)) { ok = false; break; }
-          mbar_expect_tx(&full[s], L::A_BYTES + L::B_BYTES);
-          tma_load_2d(a_tiles + s * L::A_BYTES, &map_a, &full[s], i * BK, m0);
-          tma_load_2d(b_tiles + s * L::B_BYTES, &map_w, &full[s], i * BK, n0);
+          expect(s);
+          load(a_tiles + s * L::A_BYTES, &map_a, s, i * BK, m0);
+          load(b_tiles + s * L::B_BYTES, &map_w, s, i * BK, n0);
         }
       }
     }
   } else if (warp == 1) {
-    constexpr uint32_t idesc = idesc_i8(BM, BN);
+    constexpr uint32_t idesc = idesc_i8(ROWS, BN);
     const bool one = elect_one();
     const uint64_t a_desc0 = sw128_desc(smem_u32(a_tiles)), b_desc0 = sw128_desc(smem_u32(b_tiles));
     uint32_t it = 0;
     int lt = 0;                                 // tiles of this CTA so far
-    for (int t = blockIdx.x; t < n_tiles && ok; t += gridDim.x, ++lt) {
+    for (int t = first; t < n_tiles && ok && rank == 0; t += step, ++lt) {      // (the first CTA of a pair issues for both)
       const int buf = lt & 1;
       if (lt >= 2) {
-        ok = mbar_wait(&acc_empty[buf], ((lt >> 1) & 1) ^ 1);
+        ok = PAIR ? mbar_wait_cluster(&acc_empty[buf], ((lt >> 1) & 1) ^ 1) : mbar_wait(&acc_empty[buf], ((lt >> 1) & 1) ^ 1);
         if (!ok) break;
         tc_fence_after();
       }
@@ -283,12 +330,18 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
         const uint64_t a_desc = a_desc0 + (uint32_t)s * (L::A_BYTES >> 4), b_desc = b_desc0 + (uint32_t)s * (L::B_BYTES >> 4);
         if (one) {
 #pragma unroll
-          for (int k = 0; k < BK / 32; ++k)     // 32 entries further along K: 32 bytes inside the swizzled row
-            umma_i8(acc, a_desc + (uint64_t)(k * 2), b_desc + (uint64_t)(k * 2), idesc, (i > 0 || k > 0) ? 1u : 0u);
-          umma_commit(&empty[s]);
+          for (int k = 0; k < BK / 32; ++k) {   // 32 entries further along K: 32 bytes inside the swizzled row
+            if (PAIR) umma_i8_pair(acc, a_desc + (uint64_t)(k * 2), b_desc + (uint64_t)(k * 2), idesc, (i > 0 || k > 0) ? 1u : 0u);
+            else umma_i8(acc, a_desc + (uint64_t)(k * 2), b_desc + (uint64_t)(k * 2), idesc, (i > 0 || k > 0) ? 1u : 0u);
+          }
+          if (PAIR) umma_commit_pair(&empty[s]);
+          else umma_commit(&empty[s]);
         }
       }
-      if (ok && one) umma_commit(&acc_full[buf]);
+      if (ok && one) {
+        if (PAIR) umma_commit_pair(&acc_full[buf]);
+        else umma_commit(&acc_full[buf]);
+      }
     }
   } else {
     const int quarter = warp & 3, half = warp >= 6 ? 1 : 0;       // two warps share a quarter of the lanes and take its pieces of columns in turn
@@ -297,8 +350,8 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     uint8_t* slabs = smem + L::OFF_SLAB + (warp - 2) * 4096;
     int lt = 0, sent = 0;
     pdl_wait();
-    for (int t = blockIdx.x; t < n_tiles; t += gridDim.x, ++lt) {
-      const int n0 = t % tiles_n * BN, m0 = t / tiles_n * BM, buf = lt & 1;
+    for (int t = first; t < n_tiles; t += step, ++lt) {
+      const int n0 = t % tiles_n * BN, m0 = t / tiles_n * ROWS + rank * BM, buf = lt & 1;
       const int row = m0 + quarter * 32 + lane;
       const float sa = row < M ? o.sa[row] : 0.f;
       // the tile's scales and bias, while its products run
@@ -371,7 +424,10 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_one(&acc_empty[buf]);
+      if (lane == 0) {
+        if (PAIR) mbar_arrive_cluster(&acc_empty[buf], 0);
+        else mbar_arrive_one(&acc_empty[buf]);
+      }
     }
     if (lane == 0) bulk_wait_all();
   }
@@ -380,9 +436,15 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   __syncthreads();
   tc_fence_after();
   if (*gave_up) outlast_what_is_in_flight();
+  if (PAIR) {
+    __syncwarp();
+    cluster_sync_all();                         // neither CTA goes while the other's products read its memory, or arrivals are on their way to it
+    tc_fence_after();
+  }
   if (warp == 1) {
     __syncwarp();
-    tmem_dealloc(tmem, TMEM);
+    if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM) : "memory");
+    else tmem_dealloc(tmem, TMEM);
   }
 }
 
@@ -408,12 +470,12 @@ int tensor_map(const void* p, CUtensorMapDataType type, int size, int64_t ld, in
   return KVAD_OK;
 }
 
-template <typename T, int EPI, int BN>
+template <typename T, int EPI, int BN, bool PAIR = false>
 int many(const int8_t* a, int64_t lda, const int8_t* w, const Out& o, int M, int N, int K, cudaStream_t stream) {
-  using L = Tile<BN>;
+  using L = Tile<BN, PAIR>;
   CUtensorMap ma, mw, mo;
   int rc = tensor_map(a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, lda, M, K, BM, 128, &ma);
-  if (rc == KVAD_OK) rc = tensor_map(w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, N, K, BN, 128, &mw);
+  if (rc == KVAD_OK) rc = tensor_map(w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, N, K, PAIR ? BN / 2 : BN, 128, &mw);
   if (rc != KVAD_OK) return rc;
   constexpr bool f32_out = EPI == EPI_RESIDUAL || EPI == EPI_STORE_F32 || std::is_same<T, float>::value;
   constexpr int size = f32_out ? 4 : 2;
@@ -421,19 +483,21 @@ int many(const int8_t* a, int64_t lda, const int8_t* w, const Out& o, int M, int
   if (tma_out) rc = tensor_map(o.p, f32_out ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, size, o.ld, M, N, 32, 64, &mo);
   else mo = ma;
   if (rc != KVAD_OK) return rc;
-  auto kernel = linear_int8_kernel<T, EPI, BN>;
+  auto kernel = linear_int8_kernel<T, EPI, BN, PAIR>;
   static bool configured = false;
   if (!configured) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::SMEM);
     if (e != cudaSuccess) KVAD_FAIL(KVAD_ERR_CUDA, "linear_int8: cannot reserve %zu bytes of shared memory: %s", L::SMEM, cudaGetErrorString(e));
     configured = true;
   }
-  const int64_t n_tiles = (int64_t)((N + BN - 1) / BN) * ((M + BM - 1) / BM);
+  constexpr int ROWS = PAIR ? 2 * BM : BM;
+  const int64_t n_tiles = (int64_t)((N + BN - 1) / BN) * ((M + ROWS - 1) / ROWS);
   KVAD_REQUIRE(n_tiles < (1ll << 30), "linear_int8: %lld tiles are more than one launch takes", (long long)n_tiles);
-  const int skip = g_skip_copy;
+  const int skip = g_skip_copy, most = PAIR ? sm_count() / 2 : sm_count(), at_once = (int)(n_tiles < most ? n_tiles : most);
   g_skip_copy = false;
-  const cudaError_t e = kvad_launch(kernel, dim3((unsigned)(n_tiles < sm_count() ? n_tiles : sm_count())), dim3(THREADS), L::SMEM, stream, ma, mw, mo, tma_out, o, M,
-                                    N, K, skip);
+  cudaError_t e;
+  if (PAIR) e = kvad_launch_cluster(kernel, dim3(2 * at_once), dim3(THREADS), L::SMEM, stream, dim3(2, 1, 1), ma, mw, mo, tma_out, o, M, N, K, skip);
+  else e = kvad_launch(kernel, dim3(at_once), dim3(THREADS), L::SMEM, stream, ma, mw, mo, tma_out, o, M, N, K, skip);
   if (e != cudaSuccess) KVAD_FAIL(KVAD_ERR_CUDA, "linear_int8: launch failed: %s", cudaGetErrorString(e));
   return KVAD_OK;
 }
@@ -455,14 +519,21 @@ int few(const int8_t* a, int64_t lda, const int8_t* w, const Out& o, int M, int 
   return KVAD_OK;
 }
 
-// The tile width whose waves of tiles over the SMs take the least: a wave of width BN takes BN's time, and a tile's start as much as 32 columns more; below 128
-// columns the products wait for their rows from shared memory.
-int tile_width(int M, int N) {
+// The tiles whose waves over the SMs take the least: 64, 128 or 256 columns, or 512 for pairs of CTAs on 256 x 256.  What a step of K takes a CTA is its operands' way into the SM, at some 64 bytes
+// a cycle: 375, 500 and 750 cycles for 24, 32 and 48 KB, where the products take 133, 265 and 530; one of a pair takes in 32 KB for 530 cycles' products.  The weights are those, with a
+// tile's start.  A pair's start costs a microsecond more, which short products do not win back, and where a tile's epilogue (GELU) outlasts its products a pair gains nothing
+// (us, 256 columns alone and in pairs: 8192 x 8192 x 4096 bfloat16 210 to 217, 190; 4096 x 4096 x 4096 55.0, 50.1 (128 columns 57.4); 2048 x 6400 x 1600 21.2, 19.4, with tanh GELU 23.5, 25.1;
+// 2048 x 1600 x 6400 added to the stream 23.2, 22.2; 512 x 6400 x 1600 12.9, 14.1; 1024 x 4096 x 1024 8.7, 9.2).
+int tile_width(int M, int N, int K, int epi) {
+  const int64_t sms = sm_count(), steps = (K + BK - 1) / BK, high = (M + BM - 1) / BM;
   int best = 0;
   int64_t best_cost = 0;
-  for (int bn : {256, 128, 64}) {
-    const int64_t tiles = (int64_t)((N + bn - 1) / bn) * ((M + BM - 1) / BM);
-    const int64_t cost = (tiles + sm_count() - 1) / sm_count() * ((bn < 96 ? 96 : bn) + 32);
+  for (int bn : {512, 256, 128, 64}) {
+    const bool pair = bn == 512;
+    const int64_t wide = (N + (pair ? 256 : bn) - 1) / (pair ? 256 : bn);
+    const int64_t waves = pair ? (wide * ((high + 1) / 2) + sms / 2 - 1) / (sms / 2) : (wide * high + sms - 1) / sms;
+    if (pair && (sms < 2 || waves * steps < 32 || ((epi == EPI_GELU_TANH || epi == EPI_GELU_ERF) && steps < 20))) continue;
+    const int64_t cost = waves * (pair ? 212 : (bn < 96 ? 96 : bn) + 32);
     if (best == 0 || cost < best_cost) best = bn, best_cost = cost;
   }
   return best;
@@ -471,14 +542,15 @@ int tile_width(int M, int N) {
 template <typename T, int EPI>
 int go(const int8_t* a, int64_t lda, const int8_t* w, const Out& o, int M, int N, int K, int form, cudaStream_t stream) {
   if (form == 1 || (form == 0 && M <= FEW_MAX)) return few<T, EPI>(a, lda, w, o, M, N, K, stream);
-  const int bn = form >= 64 ? form : tile_width(M, N);
+  const int bn = form >= 64 ? form : tile_width(M, N, K, EPI);
+  if (bn == 512) return many<T, EPI, 256, true>(a, lda, w, o, M, N, K, stream);
   return bn == 256 ? many<T, EPI, 256>(a, lda, w, o, M, N, K, stream) : bn == 128 ? many<T, EPI, 128>(a, lda, w, o, M, N, K, stream)
                                                                                   : many<T, EPI, 64>(a, lda, w, o, M, N, K, stream);
 }
 
 }  // namespace
 
-// `form`: 0: by the sizes; 1: the kernel of few rows (at most 16); 64, 128, 256: the kernel of many rows with tiles so wide.
+// `form`: 0: by the sizes; 1: the kernel of few rows (at most 16); 64, 128, 256: the kernel of many rows with tiles so wide; 512: tiles of 256 x 256 by pairs of CTAs.
 KVAD_EXPORT int kvad_linear_int8(int dtype, const int8_t* a, int64_t lda, const float* sa, const int8_t* w, const float* sw, const void* bias, int bias_f32,
                                  void* out, int64_t ldo, int M, int N, int K, int epi, int form, cudaStream_t stream) {
   KVAD_REQUIRE(M > 0 && N > 0 && K > 0, "linear_int8: needs rows, outputs and inputs, got %d, %d, %d", M, N, K);
@@ -486,7 +558,7 @@ KVAD_EXPORT int kvad_linear_int8(int dtype, const int8_t* a, int64_t lda, const 
   KVAD_REQUIRE(((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(w)) & 15) == 0 && lda % 16 == 0,
                "linear_int8: rows and weights must start on 16-byte boundaries");
   KVAD_REQUIRE(epi >= EPI_STORE && epi <= EPI_STORE_F32, "linear_int8: unknown epilogue %d", epi);
-  KVAD_REQUIRE(form == 0 || form == 64 || form == 128 || form == 256 || (form == 1 && M <= FEW_MAX), "linear_int8: no form %d for %d rows", form, M);
+  KVAD_REQUIRE(form == 0 || form == 64 || form == 128 || form == 256 || form == 512 || (form == 1 && M <= FEW_MAX), "linear_int8: no form %d for %d rows", form, M);
   const Out o{out, ldo, sa, sw, bias, bias_f32};
   int rc = KVAD_OK;
   const bool f32 = dtype == KVAD_DTYPE_F32;

@@ -1902,7 +1902,7 @@ class Ops:
     def linear_int8(self, a, a_scales, weight, w_scales, bias, out, epilogue: str = "store", *, form: int = 0) -> None:
         """out = epilogue((a . weight^T) * a_scales[row] * w_scales[output] + bias): rows and weights ([out_features, in_features]) as 8-bit codes with a
         scale a row of each; the sums of products are exact whole numbers.  Inputs of a multiple of 16 entries.  `form`: 0: chosen by the sizes; 1: weights
-        streamed (at most 16 rows); 64, 128, 256: the tensor-core kernel with tiles so wide."""
+        streamed (at most 16 rows); 64, 128, 256: the tensor-core kernel with tiles so wide; 512: pairs of SMs on tiles of 256 x 256."""
         _need_cuda(a, a_scales, weight, w_scales, bias, out)
         epi = EPILOGUES[epilogue]
         lda, ldo = _rows_view(a, "linear_int8 input"), _rows_view(out, "linear_int8 output")

@@ -177,7 +177,8 @@ def test_products(m, n, k, dtype, epilogue):
 
 
 # every form on its own: tiles of rows and outputs in part, more tiles than SMs, K of one block and of many
-@pytest.mark.parametrize("form,m,n,k", [(1, 1, 40, 32), (1, 13, 70, 1616), (1, 16, 40, 6416), (1, 3, 50, 2064), (64, 1, 100, 16), (64, 300, 9000, 144), (128, 40, 129, 256), (128, 500, 6000, 128), (256, 3, 3, 1040),
+@pytest.mark.parametrize("form,m,n,k", [(1, 1, 40, 32), (1, 13, 70, 1616), (1, 16, 40, 6416), (1, 3, 50, 2064), (64, 1, 100, 16), (64, 300, 9000, 144), (128, 40, 129, 256), (128, 500, 6000, 128), (256, 3, 3, 1040), (512, 3, 3, 16), (512, 300, 500, 1040), (512, 129, 70, 48),
+                                        (512, 2700, 2304, 640),
                                         (256, 1100, 5000, 272), (256, 2500, 4800, 400)])
 @pytest.mark.parametrize("dtype,epilogue", [("bfloat16", "store"), ("float32", "store"), ("bfloat16", "residual")])
 def test_products_by_form(form, m, n, k, dtype, epilogue):

@@ -28,7 +28,7 @@ def goes_without(library, count, run, out):
     assert count() == after and torch.equal(out, want) and not (out == 7).all()
 
 
-@pytest.mark.parametrize("form", [64, 128, 256])
+@pytest.mark.parametrize("form", [64, 128, 256, 512])
 def test_weights_that_never_come(form):
     g = torch.Generator(device="cuda")
     g.manual_seed(3)
