@@ -135,15 +135,18 @@ linear_int8_few_kernel(const int8_t* a, int64_t lda, const int8_t* __restrict__ 
 // Many rows
 // ---------------------------------------------------------------------------------------------------------------------------
 constexpr int BM = 128, BK = 128;             // 128 entries of K: one row of the 128-byte swizzle
-constexpr int THREADS = 320;                  // warp 0: TMA, warp 1: products and tensor memory, warps 2-9: epilogue
+// Warp 0: TMA, warp 1: products and tensor memory, the others: epilogue.  Eight of these with two slabs each, which ask for a piece of the accumulator ahead; where an entry takes some 25 instructions
+// (GELU) sixteen with one (us, eight and sixteen: 512 x 6400 x 1600 with tanh GELU 12.0, 11.4; 333 x 4096 x 1024 in 32-bit with erf 8.0, 7.5; added to the stream 2048 x 1600 x 6400 22.1, 22.4).
+__host__ __device__ constexpr int epilogue_warps(int epi) { return epi == EPI_GELU_TANH || epi == EPI_GELU_ERF ? 16 : 8; }
+constexpr int SLABS_BYTES = 8 * 4096;
 
 // PAIR: two CTAs on a tile of 256 x BN, each with 128 rows and half of the weights; the tensor cores of both read both halves.
 template <int BN, bool PAIR> struct Tile {
   static constexpr uint32_t A_BYTES = BM * BK, B_BYTES = (PAIR ? BN / 2 : BN) * BK;
   static constexpr int STAGES_RAW = 192 * 1024 / (A_BYTES + B_BYTES);
   static constexpr int STAGES = STAGES_RAW > 8 ? 8 : STAGES_RAW;
-  static constexpr uint32_t OFF_SLAB = STAGES * (A_BYTES + B_BYTES);        // two of 2 KB an epilogue warp: 32 rows x 64 bytes of output on their way out by TMA
-  static constexpr uint32_t OFF_COLS = OFF_SLAB + 8 * 4096;                 // a tile's scales and bias, an output each
+  static constexpr uint32_t OFF_SLAB = STAGES * (A_BYTES + B_BYTES);        // 2 KB each: a warp's 32 rows x 64 bytes of output on their way out by TMA
+  static constexpr uint32_t OFF_COLS = OFF_SLAB + SLABS_BYTES;                 // a tile's scales and bias, an output each
   static constexpr uint32_t OFF_BAR = OFF_COLS + 2 * BN * 4;
   static constexpr size_t SMEM = OFF_BAR + (2 * STAGES + 4) * 8 + 16;
   static_assert(SMEM <= 227 * 1024, "an SM's shared memory");
@@ -223,11 +226,11 @@ __device__ __forceinline__ void put_all(const Out& o, int row, int n, int N, con
 }
 
 template <typename T, int EPI, int BN, bool PAIR>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(64 + 32 * epilogue_warps(EPI), 1)
 linear_int8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_out,
                    int tma_out, Out o, int M, int N, int K, int skip_copy) {
   using L = Tile<BN, PAIR>;
-  constexpr int STAGES = L::STAGES, ROWS = PAIR ? 2 * BM : BM;
+  constexpr int STAGES = L::STAGES, ROWS = PAIR ? 2 * BM : BM, WARPS = epilogue_warps(EPI);
   constexpr uint32_t TMEM = 2 * BN;             // two accumulators (a power of two)
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* a_tiles = smem;
@@ -235,7 +238,7 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
   uint64_t* empty = full + STAGES;
   uint64_t* acc_full = empty + STAGES;          // [2] the accumulator is complete
-  uint64_t* acc_empty = acc_full + 2;           // [2] the eight epilogue warps have read it (of the first CTA: both CTAs')
+  uint64_t* acc_empty = acc_full + 2;           // [2] the epilogue warps have read it (of the first CTA: both CTAs')
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile uint32_t* gave_up = tmem_slot + 1;
   float* col_scale = reinterpret_cast<float*>(smem + L::OFF_COLS);
@@ -255,7 +258,7 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], PAIR ? 16 : 8);
+      mbar_init(&acc_empty[b], PAIR ? 2 * WARPS : WARPS);
     }
     *gave_up = (smem_u32(smem) & 1023) != 0;      // (the swizzle's rows start on 1024 bytes; the memory is asked for so)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -344,10 +347,11 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
       }
     }
   } else {
-    const int quarter = warp & 3, half = warp >= 6 ? 1 : 0;       // two warps share a quarter of the lanes and take its pieces of columns in turn
+    constexpr int SHARES = WARPS / 4, SLABS = SLABS_BYTES / 2048 / WARPS;       // so many warps share a quarter of the lanes and take its pieces of columns in turn
+    const int quarter = warp & 3, share = (warp - 2) >> 2;
     constexpr bool F32_OUT = EPI == EPI_RESIDUAL || EPI == EPI_STORE_F32 || std::is_same<T, float>::value;
-    constexpr int COLS = F32_OUT ? 16 : 32, PIECES = BN / COLS / 2;       // 64 bytes of output a row
-    uint8_t* slabs = smem + L::OFF_SLAB + (warp - 2) * 4096;
+    constexpr int COLS = F32_OUT ? 16 : 32, PIECES = (BN / COLS + SHARES - 1) / SHARES;       // 64 bytes of output a row
+    uint8_t* slabs = smem + L::OFF_SLAB + (warp - 2) * (SLABS * 2048);
     int lt = 0, sent = 0;
     pdl_wait();
     for (int t = first; t < n_tiles; t += step, ++lt) {
@@ -355,7 +359,7 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
       const int row = m0 + quarter * 32 + lane;
       const float sa = row < M ? o.sa[row] : 0.f;
       // the tile's scales and bias, while its products run
-      if (lt > 0) asm volatile("bar.sync 1, 256;" ::: "memory");         // the eight warps are done with those of the last
+      if (lt > 0) asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory");         // the warps are done with those of the last
       {
         const int j = threadIdx.x - 64;
         if (j < BN) {
@@ -363,36 +367,39 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
           col_bias[j] = o.bias != nullptr && n0 + j < N ? load_param(o.bias, n0 + j, o.bias_f32) : 0.f;
         }
       }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
+      asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory");
       if (ok) ok = mbar_wait(&acc_full[buf], (lt >> 1) & 1);             // (a warp whose wait runs out still meets the others above)
       if (!ok) continue;
       tc_fence_after();
-      const uint32_t acc = tmem + (uint32_t)(buf * BN) + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * COLS);
+      const uint32_t acc = tmem + (uint32_t)(buf * BN) + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(share * COLS);
       const int columns = min(BN, N - n0);
-      uint32_t r[2][COLS];
-      tmem_ask(acc, r[0]);
+      constexpr int AHEAD = SLABS - 1;
+      uint32_t r[AHEAD + 1][COLS];
+      if (AHEAD) tmem_ask(acc, r[0]);
 #pragma unroll
       for (int p = 0; p < PIECES; ++p) {
-        const int c = (2 * p + half) * COLS;
-        tmem_arrived(r[p & 1]);
-        if (p + 1 < PIECES) tmem_ask(acc + (uint32_t)((p + 1) * 2 * COLS), r[(p + 1) & 1]);      // the next piece comes while this one is worked on
+        const int c = (p * SHARES + share) * COLS;
+        if (!AHEAD && c >= columns) continue;
+        if (!AHEAD) tmem_ask(acc + (uint32_t)(p * SHARES * COLS), r[0]);
+        tmem_arrived(r[p & AHEAD]);
+        if (AHEAD && p + 1 < PIECES) tmem_ask(acc + (uint32_t)((p + 1) * SHARES * COLS), r[(p + 1) & AHEAD]);      // the next piece comes while this one is worked on
         if (c >= columns) continue;
         float v[COLS];
 #pragma unroll
         for (int j = 0; j < COLS; j += 4) {
           const float4 s4 = *reinterpret_cast<const float4*>(col_scale + c + j), b4 = *reinterpret_cast<const float4*>(col_bias + c + j);
-          v[j] = finish<EPI>(fmaf((float)(int)r[p & 1][j] * sa, s4.x, b4.x));
-          v[j + 1] = finish<EPI>(fmaf((float)(int)r[p & 1][j + 1] * sa, s4.y, b4.y));
-          v[j + 2] = finish<EPI>(fmaf((float)(int)r[p & 1][j + 2] * sa, s4.z, b4.z));
-          v[j + 3] = finish<EPI>(fmaf((float)(int)r[p & 1][j + 3] * sa, s4.w, b4.w));
+          v[j] = finish<EPI>(fmaf((float)(int)r[p & AHEAD][j] * sa, s4.x, b4.x));
+          v[j + 1] = finish<EPI>(fmaf((float)(int)r[p & AHEAD][j + 1] * sa, s4.y, b4.y));
+          v[j + 2] = finish<EPI>(fmaf((float)(int)r[p & AHEAD][j + 2] * sa, s4.z, b4.z));
+          v[j + 3] = finish<EPI>(fmaf((float)(int)r[p & AHEAD][j + 3] * sa, s4.w, b4.w));
         }
         if (!tma_out) {
           if (row < M) put_all<T, EPI, COLS>(o, row, n0 + c, N, v);
           continue;
         }
-        uint8_t* slab = slabs + (sent & 1) * 2048;
-        if (sent >= 2) {                        // its journey before has been read
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        uint8_t* slab = slabs + sent % SLABS * 2048;
+        if (sent >= SLABS) {                    // its journey before has been read
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(SLABS - 1) : "memory");
           __syncwarp();
         }
         ++sent;
@@ -496,8 +503,8 @@ int many(const int8_t* a, int64_t lda, const int8_t* w, const Out& o, int M, int
   const int skip = g_skip_copy, most = PAIR ? sm_count() / 2 : sm_count(), at_once = (int)(n_tiles < most ? n_tiles : most);
   g_skip_copy = false;
   cudaError_t e;
-  if (PAIR) e = kvad_launch_cluster(kernel, dim3(2 * at_once), dim3(THREADS), L::SMEM, stream, dim3(2, 1, 1), ma, mw, mo, tma_out, o, M, N, K, skip);
-  else e = kvad_launch(kernel, dim3(at_once), dim3(THREADS), L::SMEM, stream, ma, mw, mo, tma_out, o, M, N, K, skip);
+  if (PAIR) e = kvad_launch_cluster(kernel, dim3(2 * at_once), dim3(64 + 32 * epilogue_warps(EPI)), L::SMEM, stream, dim3(2, 1, 1), ma, mw, mo, tma_out, o, M, N, K, skip);
+  else e = kvad_launch(kernel, dim3(at_once), dim3(64 + 32 * epilogue_warps(EPI)), L::SMEM, stream, ma, mw, mo, tma_out, o, M, N, K, skip);
   if (e != cudaSuccess) KVAD_FAIL(KVAD_ERR_CUDA, "linear_int8: launch failed: %s", cudaGetErrorString(e));
   return KVAD_OK;
 }
